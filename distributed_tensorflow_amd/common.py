@@ -47,7 +47,8 @@ def set_gpu_thread_mode_and_count(flags_obj):
 
 def get_optimizer(learning_rate=0.1):
   """SGD with momentum 0.9 (`common.py:169-172`); the schedule overwrites the rate."""
-  return SGD(learning_rate=learning_rate, momentum=0.9)
+  clip = FLAGS.global_clipnorm if "global_clipnorm" in FLAGS else None
+  return SGD(learning_rate=learning_rate, momentum=0.9, global_clipnorm=clip)
 
 
 def get_callbacks(learning_rate_schedule_fn, num_images):
@@ -122,6 +123,8 @@ def define_keras_flags(dynamic_loss_scale=True):
   f.DEFINE_integer("fusion_threshold_mb", None,
                    "Gradient fusion bucket size in MB (overrides --num_packs; with neither "
                    "flag given the buckets are 25 MB).")
+  f.DEFINE_float("global_clipnorm", None, "Scale the gradient of a step down to this norm over all "
+                 "variables where it is larger (synchronous training).")
   f.DEFINE_boolean("use_hip_graph", True, "Replay the training step as a captured hipGraph "
                    "when the strategy allows it.")
   f.DEFINE_boolean("deterministic", False, "Every floating-point sum of a step in a fixed order "

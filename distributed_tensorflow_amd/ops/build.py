@@ -23,9 +23,13 @@ ARCH = "gfx950"
 # their operand-select forms have lost elements on this hardware without any error (see conv_epilogue.h).  The host pass
 # of hipcc warns that it does not know the feature.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCES = ["conv_igemm.hip", "conv_pipe.hip", "conv_halo.hip", "conv_rows.hip", "conv_wgrad_rows.hip", "conv_wgrad.hip", "bn.hip", "pool.hip", "loss.hip", "optim.hip", "dense.hip",
+SOURCES = ["conv_igemm.hip", "conv_pipe.hip", "conv_halo.hip", "conv_rows.hip", "conv_wgrad_rows.hip", "conv_wgrad.hip", "bn.hip", "pool.hip", "loss.hip", "optim.hip", "dense.hip", "residual_norm.hip",
+           "grad_clip.hip",
            "rccl_comm.cpp", "bindings.cpp"]
 HEADERS = ["common.h", "conv_params.h", "conv_epilogue.h", "elementwise.h", "rccl_comm.h"]
+# headers of one kernel file and the bindings
+OWN_HEADERS = {"residual_norm.hip": ["residual_norm.h"], "grad_clip.hip": ["grad_clip.h"],
+               "bindings.cpp": ["residual_norm.h", "grad_clip.h"]}
 
 
 def so_path() -> str:
@@ -46,7 +50,7 @@ def _stale(target, deps):
 
 def _compile(src, force):
   obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
-  deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS]
+  deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS + OWN_HEADERS.get(src, [])]
   if not force and not _stale(obj, deps):
     return obj, False
   cmd = ["hipcc", "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden"] + NO_PACKED_FP32 + [

@@ -23,7 +23,9 @@
 #include "common.h"
 #include "conv_params.h"
 #include "elementwise.h"
+#include "grad_clip.h"
 #include "rccl_comm.h"
+#include "residual_norm.h"
 
 namespace py = pybind11;
 using Launch = std::function<void(hipStream_t)>;
@@ -160,6 +162,38 @@ WgradParams wgrad_from_dict(const py::dict& d) {
   p.divOH = make_fastdiv((uint32_t)p.OH);
   p.divCpad = make_fastdiv((uint32_t)p.Cpad);
   p.divTJpad = make_fastdiv((uint32_t)p.TJpad);
+  return p;
+}
+
+ResidualNormParams residual_norm_from_dict(const py::dict& d, bool backward) {
+  ResidualNormParams p;
+  p.dt = get_or<int>(d, "dt", DT_BF16);
+  p.P = get<int>(d, "P"); p.C = get<int>(d, "C");
+  p.layer = get_or<int>(d, "layer", 0); p.sigmoid = get_or<int>(d, "sigmoid", 0);
+  p.scale = get_or<float>(d, "scale", 1.f); p.eps = get_or<float>(d, "eps", 1e-6f);
+  p.y = ptr<const void>(d, "y", false); p.ldy = get_or<int64_t>(d, "ldy", p.C);
+  p.gate = ptr<const void>(d, "gate", false); p.ldgate = get_or<int64_t>(d, "ldgate", p.C);
+  // a gate row per `group_rows` rows (fp32), or 0: one per row in the rows' own type
+  p.group_rows = get_or<int>(d, "group_rows", 0);
+  p.gate_mode = !p.gate ? GATE_NONE : p.group_rows > 0 ? GATE_GROUP : GATE_ELEMENT;
+  p.post_gamma = ptr<const float>(d, "post_gamma", false); p.post_beta = ptr<const float>(d, "post_beta", false);
+  p.pre_gamma = ptr<const float>(d, "pre_gamma", false); p.pre_beta = ptr<const float>(d, "pre_beta", false);
+  if (!backward) {
+    p.x = ptr<const void>(d, "x"); p.ldx = get_or<int64_t>(d, "ldx", p.C);
+    p.h = ptr<void>(d, "h", p.y != nullptr); p.z = ptr<void>(d, "z", p.pre_gamma != nullptr);
+    return p;
+  }
+  p.dh = ptr<const void>(d, "dh", false); p.lddh = get_or<int64_t>(d, "lddh", p.C);
+  p.dz = ptr<const void>(d, "dz", p.pre_gamma != nullptr); p.lddz = get_or<int64_t>(d, "lddz", p.C);
+  p.x = ptr<const void>(d, "h", p.pre_gamma != nullptr); p.ldx = get_or<int64_t>(d, "ldh", p.C);
+  p.dx = ptr<void>(d, "dx"); p.dy = ptr<void>(d, "dy", p.y != nullptr);
+  p.dgate = ptr<void>(d, "dgate", p.gate != nullptr);
+  p.dpost_gamma = ptr<float>(d, "dpost_gamma", p.post_gamma != nullptr);
+  p.dpost_beta = ptr<float>(d, "dpost_beta", p.post_beta != nullptr);
+  p.dpre_gamma = ptr<float>(d, "dpre_gamma", p.pre_gamma != nullptr);
+  p.dpre_beta = ptr<float>(d, "dpre_beta", p.pre_beta != nullptr);
+  p.ws = ptr<float>(d, "ws", false);
+  if (!p.ws && residual_norm_workspace_floats(p)) throw std::invalid_argument("missing tensor 'ws'");
   return p;
 }
 
@@ -360,6 +394,21 @@ Launch make_op(const std::string& kind, const py::dict& d, bool planned = false)
     auto skip = ptr<const float>(d, "skip", false);     // device [skip flag, inverse loss scale]
     const int um = get_or<int>(d, "use_momentum", mom != 0.f ? 1 : 0);
     return [=](hipStream_t s) { launch_sgd_momentum_l2(p, g, v, l2, n, lr, mom, gs, um, hyper, skip, s); };
+  }
+  if (kind == "clipped_sgd") {
+    auto p = ptr<float>(d, "p"); auto g = ptr<const float>(d, "g"); auto v = ptr<float>(d, "v");
+    auto l2 = ptr<const float>(d, "l2x2"); auto skip = ptr<const float>(d, "skip", false);
+    auto ws = ptr<double>(d, "ws"); auto norm = ptr<float>(d, "norm", false);    // clipped_sgd_blocks(n) doubles
+    const size_t n = get<size_t>(d, "n");
+    const float lr = get<float>(d, "lr"), mom = get<float>(d, "momentum"), clip = get<float>(d, "clip");
+    const float gs = get_or<float>(d, "grad_scale", 1.f);
+    return [=](hipStream_t s) { launch_clipped_sgd_momentum_l2(p, g, v, l2, n, lr, mom, gs, clip, skip, ws, norm, s); };
+  }
+  if (kind == "residual_norm_fwd" || kind == "residual_norm_bwd") {
+    const bool backward = kind == "residual_norm_bwd";
+    const ResidualNormParams p = residual_norm_from_dict(d, backward);
+    if (backward) return [p](hipStream_t s) { launch_residual_norm_bwd(p, s); };
+    return [p](hipStream_t s) { launch_residual_norm_fwd(p, s); };
   }
   if (kind == "dense_fwd") {
     auto x = ptr<const void>(d, "x"); auto w = ptr<const float>(d, "w");
@@ -758,6 +807,39 @@ PYBIND11_MODULE(_dtf_native, m) {
   m.def("bn_workspace_floats", []() { return bn_workspace_floats(); });
   m.def("bn_tail_floats", []() { return bn_tail_floats(); });
   m.def("bn_fold_desc_size", []() { return bn_fold_desc_size(); });
+  m.def("residual_norm_workspace_floats", [](int P, int C, int group_rows) {
+    ResidualNormParams p;
+    p.P = P; p.C = C; p.group_rows = group_rows;
+    p.gate_mode = group_rows > 0 ? GATE_GROUP : GATE_NONE;
+    return residual_norm_workspace_floats(p);
+  }, "Floats that residual_norm_bwd keeps its partial sums in; group_rows: rows that share a gate row, or 0");
+  m.def("clipped_sgd_blocks", &clipped_sgd_blocks);
+  m.attr("RESIDUAL_NORM_MAX_C") = RESIDUAL_NORM_MAX_C;
+  py::class_<ClipList>(m, "ClipList")
+      .def(py::init([](const std::vector<uintptr_t>& in, const std::vector<uintptr_t>& out,
+                       const std::vector<int64_t>& n, const std::vector<int>& dt) {
+             if (n.size() != in.size() || dt.size() != in.size() || (!out.empty() && out.size() != in.size()))
+               throw std::invalid_argument("ClipList: lists of different lengths");
+             std::vector<ClipTensor> t(in.size());
+             for (size_t i = 0; i < in.size(); ++i)
+               t[i] = ClipTensor{reinterpret_cast<const void*>(in[i]),
+                                 out.empty() ? nullptr : reinterpret_cast<void*>(out[i]), n[i], dt[i]};
+             return new ClipList(t);
+           }), py::arg("in"), py::arg("out"), py::arg("n"), py::arg("dt"))
+      .def_property_readonly("workspace_doubles", &ClipList::workspace_doubles)
+      .def("global_norm", [](const ClipList& l, uintptr_t ws, uintptr_t norm, uintptr_t s) {
+             auto* w = reinterpret_cast<double*>(ws);
+             l.norm(w, reinterpret_cast<hipStream_t>(s));
+             l.finish(w, reinterpret_cast<float*>(norm), reinterpret_cast<hipStream_t>(s));
+             check_launch(); },
+           py::arg("ws"), py::arg("norm"), py::arg("stream"))
+      .def("clip", [](const ClipList& l, uintptr_t ws, uintptr_t use_norm, float clip, uintptr_t norm, uintptr_t s) {
+             auto* w = reinterpret_cast<double*>(ws);
+             if (!use_norm) l.norm(w, reinterpret_cast<hipStream_t>(s));
+             l.scale(w, reinterpret_cast<const float*>(use_norm), clip, reinterpret_cast<float*>(norm),
+                     reinterpret_cast<hipStream_t>(s));
+             check_launch(); },
+           py::arg("ws"), py::arg("use_norm"), py::arg("clip"), py::arg("norm"), py::arg("stream"));
   m.attr("PACK_PER_BLOCK") = 256 * 8;
   m.attr("arch") = "gfx950";
   py::class_<Plan>(m, "Plan")

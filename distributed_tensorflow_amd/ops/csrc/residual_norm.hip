@@ -1,0 +1,602 @@
+// The seam between two residual blocks, forward and backward.
+//
+//   n = N(y) * post_gamma + post_beta          (n = y without post_gamma)
+//   h = x + scale * a(gate) * n                (a: identity or sigmoid; h = x without y)
+//   z = N(h) * pre_gamma + pre_beta            (the next block's input; none without pre_gamma)
+//
+// N normalises a row over its C channels: v / sqrt(mean v^2 + eps), or with `layer` (v - mean) / sqrt(var + eps).
+// Rows are pixels of an NHWC activation or tokens.  The work is a handful of operations per element, so memory
+// bounds it: every tensor is read once and written once, a row stays in registers (fp32) between its two
+// normalisations, and nothing but results goes back to memory.  z is taken from the unrounded h.
+//
+// Split: a lane owns eight consecutive channels (16 bytes of a 16-bit row).  Rows of up to 512 channels share a
+// wave (2 .. 64 lanes a row, sums by butterfly); wider rows take as many waves as they need, up to eight with one
+// or two chunks of eight channels a lane, and join their sums through LDS.
+//
+// Loads take any alignment (rows of odd length start anywhere); the last, partial chunk of a row goes element by element.
+#include <stdexcept>
+
+#include "residual_norm.h"
+
+namespace {
+
+// 16 bytes at the alignment of their elements: the memory system takes any address, one load all the same
+struct __attribute__((packed, aligned(2))) Any16 { u32x4 v; };
+struct __attribute__((packed, aligned(4))) Any16F { f32x4 v; };
+
+// Eight channels from `c` on of the row at `p`, as floats; what lies past channel C - 1 is zero.
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, int c, int C, float* f) {
+  if (c + 8 <= C) {
+    Raw8<DT> r;
+    if constexpr (DT == DT_F32) {
+      r.lo = reinterpret_cast<const Any16F*>(p + c)->v;
+      r.hi = reinterpret_cast<const Any16F*>(p + c + 4)->v;
+    } else {
+      r.v = reinterpret_cast<const Any16*>(p + c)->v;
+    }
+    unpack8<DT>(r, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = c + j < C ? to_f<DT>(p[c + j]) : 0.f;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(typename Elem<DT>::T* p, int c, int C, const float* f) {
+  if (c + 8 <= C) {
+    if constexpr (DT == DT_F32) {
+      reinterpret_cast<Any16F*>(p + c)->v = f32x4{f[0], f[1], f[2], f[3]};
+      reinterpret_cast<Any16F*>(p + c + 4)->v = f32x4{f[4], f[5], f[6], f[7]};
+    } else {
+      u32x4 v;
+      v.x = pack2<DT>(f[0], f[1]); v.y = pack2<DT>(f[2], f[3]);
+      v.z = pack2<DT>(f[4], f[5]); v.w = pack2<DT>(f[6], f[7]);
+      reinterpret_cast<Any16*>(p + c)->v = v;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < C) p[c + j] = from_f<DT>(f[j]);
+  }
+}
+
+// fp32 rows take the library's exponential and a true division, 16-bit rows the hardware's (their error, a few
+// 2^-22, vanishes in the rounding of the result).
+template <int DT>
+__device__ __forceinline__ float sigmoid_f(float g) {
+  if constexpr (DT == DT_F32) return 1.f / (1.f + expf(-g));
+  else return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+}
+
+// Sums of N values over the lanes of a row, given to all of them.  LPR lanes of a wave hold a narrow row; a wide one
+// has `waves` whole waves, joined through the half `turn & 1` of `red`: the barrier of the next sum separates this
+// sum's reads from the writes after next.
+template <int LPR, bool WIDE, int N>
+__device__ __forceinline__ void row_sums(float* v, float (*red)[4][8], int waves, int& turn) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  if constexpr (WIDE) {
+    float (*mine)[8] = red[turn & 1];
+    ++turn;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) mine[i][threadIdx.x >> 6] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+      for (int w = 0; w < waves; ++w) s += mine[i][w];
+      v[i] = s;
+    }
+  }
+}
+
+// Centres `v` (layer) and returns 1 / sqrt(mean square + eps) of the row.
+template <int LPR, bool WIDE, int K>
+__device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, float inv_c, int layer, float eps,
+                                           float (*red)[4][8], int waves, int& turn) {
+  float s[1];
+  if (layer) {
+    s[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[0] += v[k][j];
+    row_sums<LPR, WIDE, 1>(s, red, waves, turn);
+    const float mean = s[0] * inv_c;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = c[k] + j < C ? v[k][j] - mean : 0.f;
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[0] += v[k][j] * v[k][j];
+  row_sums<LPR, WIDE, 1>(s, red, waves, turn);
+  return 1.f / sqrtf(s[0] * inv_c + eps);
+}
+
+template <int DT, int LPR, bool WIDE, int K>
+__global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNormParams p) {
+  typedef typename Elem<DT>::T T;
+  __shared__ float red[2][4][8];
+  int turn = 0;
+  const int lanes = WIDE ? (int)blockDim.x : LPR;
+  const int waves = WIDE ? (int)(blockDim.x >> 6) : 1;
+  const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x % LPR);
+  const int slots = WIDE ? 1 : 256 / LPR;
+  const int slot = WIDE ? 0 : (int)(threadIdx.x / LPR);
+  const int C = p.C;
+  const float inv_c = 1.f / (float)C;
+  int c[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) c[k] = (lane + k * lanes) * 8;
+  // every lane of a wave walks the same number of passes (the sums need all of them); rows past the end are masked
+  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.P; base += (int64_t)gridDim.x * slots) {
+    const int64_t row = base + slot;
+    const bool live = row < p.P;
+    const int Cr = live ? C : 0;       // a dead row has no channels: nothing is read or written for it
+    const int64_t r = live ? row : 0;
+    float h[K][8], v[K][8];
+#pragma unroll
+    for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], Cr, h[k]);
+    if (p.y) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], Cr, v[k]);
+      float g[K][8];
+      if (p.gate_mode == GATE_ELEMENT) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], Cr, g[k]);
+      } else if (p.gate_mode == GATE_GROUP) {
+        const float* row_g = reinterpret_cast<const float*>(p.gate) + (r / p.group_rows) * p.ldgate;
+#pragma unroll
+        for (int k = 0; k < K; ++k) load8<DT_F32>(row_g, c[k], Cr, g[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[k][j] = 1.f;
+      }
+      if (p.sigmoid) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
+      }
+      if (p.post_gamma) {
+        const float rs = normalise<LPR, WIDE, K>(v, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float w[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          load8<DT_F32>(p.post_gamma, c[k], C, w);
+          if (p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, b);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * rs * w[j] + b[j];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[k][j] += p.scale * (g[k][j] * v[k][j]);
+        store8<DT>(reinterpret_cast<T*>(p.h) + r * C, c[k], Cr, h[k]);
+      }
+    }
+    if (p.pre_gamma) {
+      const float rs = normalise<LPR, WIDE, K>(h, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float w[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        load8<DT_F32>(p.pre_gamma, c[k], C, w);
+        if (p.pre_beta) load8<DT_F32>(p.pre_beta, c[k], C, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[k][j] = h[k][j] * rs * w[j] + b[j];
+        store8<DT>(reinterpret_cast<T*>(p.z) + r * C, c[k], Cr, h[k]);
+      }
+    }
+  }
+}
+
+// ---- backward ----------------------------------------------------------------------------------
+//   H  = dh + r_h (dz' - [mean dz'] - hat_h mean(dz' hat_h))        dz' = dz * pre_gamma,  hat_h = N(h)
+//   dx = H        up = scale * H        dgate = up * n * a'(gate)   dn = up * a(gate)
+//   dy = r_y (t - [mean t] - hat_y mean(t hat_y))                   t = dn * post_gamma,   hat_y = N(y)
+//   dpre_gamma = sum dz hat_h   dpre_beta = sum dz   dpost_gamma = sum dn hat_y   dpost_beta = sum dn
+// (the bracketed means only with `layer`).  The statistics are taken again from h and y, which are in registers
+// anyway: two sums more per row instead of saved tensors that could belong to another call.
+// A lane keeps its channels for all of its block's rows, so the sums over rows are registers; blocks leave one row of
+// partial sums each and finish_kernel adds them in a fixed order (no atomics: the same bits every time).
+//
+// A block's rows lie in one group (of rows that share a gate row), or it owns whole groups; where a group has fewer
+// rows than the block has row slots, every slot owns whole groups of its own (`own_groups`).
+
+struct BwdPlan {
+  int blocks;        // grid
+  int parts;         // blocks per group
+  int groups;        // groups of rows (1 without a group gate)
+  int group_rows;
+  int part_rows;     // rows of a group per part
+  int own_groups;    // each row slot takes whole groups
+};
+
+int narrow_lanes(int C) {       // lanes a row of up to 512 channels
+  int l = 2;
+  while (l * 8 < C) l *= 2;
+  return l;
+}
+
+int fwd_blocks(int P, int slots) {
+  const int64_t want = ((int64_t)P + slots - 1) / slots;
+  return (int)(want < 8192 ? want : 8192);
+}
+
+BwdPlan plan_bwd(const ResidualNormParams& p) {
+  BwdPlan b;
+  const bool grouped = p.gate_mode == GATE_GROUP;
+  b.group_rows = grouped ? p.group_rows : p.P;
+  b.groups = p.P / b.group_rows;
+  const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
+  const int want = 1024;
+  b.own_groups = grouped && slots > 1 && b.group_rows < 4 * slots;
+  if (b.own_groups) {
+    const int sets = (b.groups + slots - 1) / slots;
+    b.blocks = sets < want ? sets : want;
+    b.parts = 1;
+    b.part_rows = b.group_rows;
+    return b;
+  }
+  if (b.groups >= want) {
+    b.blocks = want;
+    b.parts = 1;
+  } else {
+    int most = (b.group_rows + slots - 1) / slots;         // a part has work for every slot
+    b.parts = want / b.groups;
+    if (b.parts > most) b.parts = most;
+    b.blocks = b.groups * b.parts;
+  }
+  b.part_rows = (b.group_rows + b.parts - 1) / b.parts;
+  return b;
+}
+
+// Partial sums: [vector][block][C]; which vectors are kept goes by the gradients asked for.
+struct Partials {
+  float* row[5];      // dpre_gamma, dpre_beta, dpost_gamma, dpost_beta, dgate
+};
+
+template <int DT, int LPR, bool WIDE, int K>
+__global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
+                                                               const Partials part) {
+  typedef typename Elem<DT>::T T;
+  __shared__ float red[2][4][8];
+  __shared__ float join[WIDE ? 1 : 256 * 8];
+  int turn = 0;
+  const int lanes = WIDE ? (int)blockDim.x : LPR;
+  const int waves = WIDE ? (int)(blockDim.x >> 6) : 1;
+  const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x % LPR);
+  const int slots = WIDE ? 1 : 256 / LPR;
+  const int slot = WIDE ? 0 : (int)(threadIdx.x / LPR);
+  const int C = p.C;
+  const float inv_c = 1.f / (float)C;
+  int c[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) c[k] = (lane + k * lanes) * 8;
+  float acc[5][K][8];
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][k][j] = 0.f;
+  float pw[K][8], pb[K][8], qw[K][8];     // post_gamma, post_beta, pre_gamma
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pw[k][j] = pb[k][j] = qw[k][j] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (p.post_gamma) load8<DT_F32>(p.post_gamma, c[k], C, pw[k]);
+    if (p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, pb[k]);
+    if (p.pre_gamma) load8<DT_F32>(p.pre_gamma, c[k], C, qw[k]);
+  }
+  // the sets of groups this block works on, and the rows of a group that are its own
+  const int per_set = plan.own_groups ? slots : 1;
+  const int first_set = plan.parts > 1 ? (int)blockIdx.x / plan.parts : (int)blockIdx.x;
+  const int stride_set = plan.parts > 1 ? plan.groups : (int)gridDim.x;      // parts > 1: one group a block
+  const int sets = (plan.groups + per_set - 1) / per_set;
+  const int row0 = plan.parts > 1 ? ((int)blockIdx.x % plan.parts) * plan.part_rows : 0;
+  const int row1 = min(row0 + plan.part_rows, plan.group_rows);
+  const int step = plan.own_groups ? 1 : slots;
+  for (int set = first_set; set < sets; set += stride_set) {
+    const int group = plan.own_groups ? set * slots + slot : set;
+    const bool group_live = group < plan.groups;
+    float g[K][8];
+    if (p.gate_mode == GATE_GROUP) {
+      const float* row_g = reinterpret_cast<const float*>(p.gate) + (int64_t)(group_live ? group : 0) * p.ldgate;
+#pragma unroll
+      for (int k = 0; k < K; ++k) load8<DT_F32>(row_g, c[k], C, g[k]);
+    }
+    for (int rr = row0; rr < row1; rr += step) {
+      const int in_group = plan.own_groups ? rr : rr + slot;
+      const bool live = group_live && in_group < row1;
+      const int Cr = live ? C : 0;
+      const int64_t r = live ? (int64_t)group * plan.group_rows + in_group : 0;
+      float up[K][8], dz[K][8], h[K][8], v[K][8], a[K][8], slope[K][8];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (p.dh) load8<DT>(reinterpret_cast<const T*>(p.dh) + r * p.lddh, c[k], Cr, up[k]);
+        if (p.dz) load8<DT>(reinterpret_cast<const T*>(p.dz) + r * p.lddz, c[k], Cr, dz[k]);
+        if (p.dz) load8<DT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], Cr, h[k]);
+        if (p.y) load8<DT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], Cr, v[k]);
+      }
+      if (p.gate_mode == GATE_ELEMENT) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], Cr, a[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[k][j] = p.gate_mode == GATE_GROUP ? g[k][j] : 1.f;
+      }
+      if (!p.dh) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) up[k][j] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (p.sigmoid) {
+            a[k][j] = sigmoid_f<DT>(a[k][j]);
+            slope[k][j] = a[k][j] * (1.f - a[k][j]);
+          } else {
+            slope[k][j] = 1.f;
+          }
+        }
+      if (p.dz) {
+        const float rs = normalise<LPR, WIDE, K>(h, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            h[k][j] *= rs;
+            const float d = dz[k][j] * qw[k][j];
+            s[0] += d * h[k][j];
+            s[1] += d;
+          }
+        row_sums<LPR, WIDE, 2>(s, red, waves, turn);
+        const float m_dot = s[0] * inv_c, m_d = p.layer ? s[1] * inv_c : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            up[k][j] += rs * (dz[k][j] * qw[k][j] - m_d - h[k][j] * m_dot);
+            acc[0][k][j] += dz[k][j] * h[k][j];
+            acc[1][k][j] += dz[k][j];
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) store8<DT>(reinterpret_cast<T*>(p.dx) + r * C, c[k], Cr, up[k]);
+      if (!p.y) continue;
+      float rs = 1.f;
+      if (p.post_gamma) rs = normalise<LPR, WIDE, K>(v, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float dg[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          // a dead row or channel has h, dz, dh, y of zero; its `up` is not (the mean of dz' under `layer`)
+          const float u = c[k] + j < Cr ? p.scale * up[k][j] : 0.f;
+          const float hat = v[k][j] * rs;
+          const float n = p.post_gamma ? hat * pw[k][j] + pb[k][j] : hat;
+          const float dn = u * a[k][j];
+          dg[j] = u * n;
+          acc[4][k][j] += dg[j];
+          dg[j] *= slope[k][j];
+          acc[2][k][j] += dn * hat;
+          acc[3][k][j] += dn;
+          v[k][j] = hat;
+          up[k][j] = p.post_gamma ? dn * pw[k][j] : dn;
+          s[0] += up[k][j] * hat;
+          s[1] += up[k][j];
+        }
+        if (p.gate_mode == GATE_ELEMENT) store8<DT>(reinterpret_cast<T*>(p.dgate) + r * C, c[k], Cr, dg);
+      }
+      if (p.post_gamma) {
+        row_sums<LPR, WIDE, 2>(s, red, waves, turn);
+        const float m_dot = s[0] * inv_c, m_d = p.layer ? s[1] * inv_c : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) up[k][j] = rs * (up[k][j] - m_d - v[k][j] * m_dot);
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) store8<DT>(reinterpret_cast<T*>(p.dy) + r * C, c[k], Cr, up[k]);
+    }
+    if (p.gate_mode == GATE_GROUP && plan.parts == 1) {
+      // whole groups: the gate's gradient is complete here
+      if (!WIDE && !plan.own_groups) {
+        static_assert(WIDE || K == 1, "narrow rows have one chunk a lane");
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) join[slot * LPR * 8 + lane * 8 + j] = acc[4][0][j];
+        __syncthreads();
+        for (int col = threadIdx.x; col < C; col += 256) {
+          float sum = 0.f;
+          for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + col];
+          float f = 1.f;
+          if (p.sigmoid) {
+            const float sg = sigmoid_f<DT>(reinterpret_cast<const float*>(p.gate)[(int64_t)group * p.ldgate + col]);
+            f = sg * (1.f - sg);
+          }
+          reinterpret_cast<float*>(p.dgate)[(int64_t)group * C + col] = sum * f;
+        }
+      } else if (group_live) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float dg[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float f = 1.f;
+            if (p.sigmoid) {
+              const float sg = sigmoid_f<DT>(g[k][j]);
+              f = sg * (1.f - sg);
+            }
+            dg[j] = acc[4][k][j] * f;
+          }
+          store8<DT_F32>(reinterpret_cast<float*>(p.dgate) + (int64_t)group * C, c[k], C, dg);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[4][k][j] = 0.f;
+    }
+  }
+  // the block's row of partial sums
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    if (!part.row[i]) continue;
+    float* out = part.row[i] + (int64_t)blockIdx.x * C;
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) store8<DT_F32>(out, c[k], C, acc[i][k]);
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) join[slot * LPR * 8 + lane * 8 + j] = acc[i][0][j];
+      __syncthreads();
+      for (int col = threadIdx.x; col < C; col += 256) {
+        float sum = 0.f;
+        for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + col];
+        out[col] = sum;
+      }
+    }
+  }
+}
+
+// Sums the blocks' partial rows: vector blockIdx.y, 32 columns a block, 32 slices of the rows.  For the gate's
+// gradient (`of_group`, vector 4) the rows of one group are `parts` consecutive ones and blockIdx.z is the group.
+struct Finish {
+  const float* from[5];
+  float* to[5];
+  const float* gate;
+  int64_t ldgate;
+  int C, rows, parts, sigmoid;
+};
+
+template <int DT>
+__global__ __launch_bounds__(1024) void finish_kernel(const Finish f, int first) {
+  __shared__ float join[32][33];
+  const int i = first + blockIdx.y;
+  const int rows = i == 4 ? f.parts : f.rows, group = blockIdx.z;
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  float sum = 0.f;
+  if (f.to[i] && col < f.C) {
+    const float* from = f.from[i] + (int64_t)group * f.parts * f.C + col;
+#pragma unroll 8
+    for (int r = slice; r < rows; r += 32) sum += from[(int64_t)r * f.C];
+  }
+  join[slice][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (slice == 0 && f.to[i] && col < f.C) {
+    sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) sum += join[q][threadIdx.x];
+    if (i == 4 && f.sigmoid) {
+      const float sg = sigmoid_f<DT>(f.gate[(int64_t)group * f.ldgate + col]);
+      sum *= sg * (1.f - sg);
+    }
+    f.to[i][(int64_t)group * f.C + col] = sum;
+  }
+}
+
+void check(const ResidualNormParams& p) {
+  if (p.C < 1 || p.C > RESIDUAL_NORM_MAX_C) throw std::invalid_argument("residual_norm: 1 to 8192 channels");
+  if (p.P < 0 || p.P > 0x7fff0000) throw std::invalid_argument("residual_norm: too many rows");
+  if (!(p.eps > 0.f)) throw std::invalid_argument("residual_norm: eps has to be positive");   // rows of zeros
+  if (p.gate_mode == GATE_GROUP && (p.group_rows < 1 || p.P % p.group_rows))
+    throw std::invalid_argument("residual_norm: the rows of a gate's groups have to divide the rows");
+  if ((p.post_gamma || p.gate_mode != GATE_NONE) && !p.y)
+    throw std::invalid_argument("residual_norm: a gate or post_gamma without y");
+  if ((p.post_beta && !p.post_gamma) || (p.pre_beta && !p.pre_gamma) || (!p.layer && (p.post_beta || p.pre_beta)))
+    throw std::invalid_argument("residual_norm: a beta goes with its gamma and with norm='layer'");
+}
+
+// (lanes per row, wide, chunks per lane) by the row's length alone: eight channels a lane while that takes at most
+// 512 threads, sixteen above.
+#define DTF_ROW_SWITCH(C, ...)                                                                     \
+  do {                                                                                             \
+    if ((C) <= 16) { constexpr int LPR = 2, K = 1; constexpr bool WIDE = false; __VA_ARGS__; }      \
+    else if ((C) <= 32) { constexpr int LPR = 4, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
+    else if ((C) <= 64) { constexpr int LPR = 8, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
+    else if ((C) <= 128) { constexpr int LPR = 16, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
+    else if ((C) <= 256) { constexpr int LPR = 32, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
+    else if ((C) <= 512) { constexpr int LPR = 64, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
+    else if ((C) <= 4096) { constexpr int LPR = 64, K = 1; constexpr bool WIDE = true; __VA_ARGS__; } \
+    else { constexpr int LPR = 64, K = 2; constexpr bool WIDE = true; __VA_ARGS__; }                \
+  } while (0)
+
+int wide_threads(int C) {
+  const int per_wave = C <= 4096 ? 512 : 1024;
+  return 64 * ((C + per_wave - 1) / per_wave);
+}
+
+}  // namespace
+
+size_t residual_norm_workspace_floats(const ResidualNormParams& p) {
+  if (p.P <= 0 || p.C < 1 || (p.gate_mode == GATE_GROUP && p.group_rows < 1)) return 0;
+  return (size_t)5 * plan_bwd(p).blocks * p.C;
+}
+
+void launch_residual_norm_fwd(const ResidualNormParams& p, hipStream_t s) {
+  check(p);
+  if (p.P == 0) return;
+  const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
+  const int blocks = fwd_blocks(p.P, p.C <= 512 ? 256 / narrow_lanes(p.C) : 1);
+  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((fwd_kernel<DT, LPR, WIDE, K>), dim3(blocks), dim3(threads),
+                                                             0, s, p)));
+}
+
+void launch_residual_norm_bwd(const ResidualNormParams& p, hipStream_t s) {
+  check(p);
+  if (p.P == 0) return;         // the caller clears the vectors' gradients
+  if ((p.dz != nullptr) != (p.pre_gamma != nullptr))
+    throw std::invalid_argument("residual_norm_grad: dz goes with pre_gamma");
+  if (!p.dz && !p.dh) throw std::invalid_argument("residual_norm_grad: neither dh nor dz");
+  const BwdPlan plan = plan_bwd(p);
+  const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
+  float* to[5] = {p.dpre_gamma, p.dpre_beta, p.dpost_gamma, p.dpost_beta, nullptr};
+  if (p.gate_mode == GATE_GROUP && plan.parts > 1) to[4] = reinterpret_cast<float*>(p.dgate);
+  Partials part;
+  Finish f;
+  bool any = false;
+  for (int i = 0; i < 5; ++i) {
+    part.row[i] = to[i] ? p.ws + (size_t)i * plan.blocks * p.C : nullptr;
+    f.from[i] = part.row[i];
+    f.to[i] = to[i];
+    any = any || to[i];
+  }
+  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((bwd_kernel<DT, LPR, WIDE, K>), dim3(plan.blocks),
+                                                             dim3(threads), 0, s, p, plan, part)));
+  if (!any) return;
+  f.gate = reinterpret_cast<const float*>(p.gate);
+  f.ldgate = p.ldgate;
+  f.C = p.C;
+  f.rows = plan.blocks;
+  f.parts = plan.parts;
+  f.sigmoid = p.sigmoid;
+  const int cols = (p.C + 31) / 32;
+  if (to[0] || to[1] || to[2] || to[3])
+    DTF_DT_SWITCH(p.dt, hipLaunchKernelGGL(finish_kernel<DT>, dim3(cols, 4, 1), dim3(1024), 0, s, f, 0));
+  if (to[4])
+    DTF_DT_SWITCH(p.dt, hipLaunchKernelGGL(finish_kernel<DT>, dim3(cols, 1, plan.groups), dim3(1024), 0, s, f, 4));
+}

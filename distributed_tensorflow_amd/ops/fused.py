@@ -7,9 +7,12 @@ library fallback on the device path.
 """
 from __future__ import annotations
 
+from typing import Dict, Optional, Sequence
+
 import torch
 
-__all__ = ["sgd_momentum_l2"]
+__all__ = ["sgd_momentum_l2", "clipped_sgd_momentum_l2", "TensorTable", "global_norm", "clip_by_global_norm",
+           "residual_norm", "residual_norm_grad"]
 
 
 def sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity: torch.Tensor,
@@ -35,3 +38,396 @@ def sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity: torch.T
       params.add_(velocity)
     else:
       params.add_(g, alpha=-lr)
+
+# ---- the seam between two residual blocks ----------------------------------------------------------
+
+MAX_CHANNELS = 8192      # of the native kernels
+
+
+def _pitch(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
+  """Elements from one row of `t` to the next; rows are everything but the last dimension."""
+  if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    raise ValueError("%s: %s %s on %s, but the rows are %s %s on %s" % (
+        name, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
+  return _row_pitch(name, t)
+
+
+def _row_pitch(name: str, t: torch.Tensor) -> int:
+  channels = t.shape[-1]
+  if t.is_contiguous():
+    return channels
+  if channels > 1 and t.stride(-1) != 1:
+    raise ValueError("%s: the channels of a row have to lie next to each other" % name)
+  if t.dim() == 1:
+    return channels
+  pitch = t.stride(-2)
+  for d in range(t.dim() - 2):      # the rows in front have to continue at the same pitch
+    if t.shape[d] > 1 and t.stride(d) != pitch * t.shape[d + 1:-1].numel():
+      raise ValueError("%s: its rows lie at different distances" % name)
+  return pitch
+
+
+class _Seam:
+  """Checked arguments of `residual_norm` and `residual_norm_grad`."""
+
+  __slots__ = ("rows", "channels", "group_rows", "sigmoid", "layer", "gate_pitch")
+
+  def __init__(self, like, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps):
+    if like.dim() < 1 or like.shape[-1] < 1:
+      raise ValueError("rows of at least one channel, got %s" % (tuple(like.shape),))
+    if like.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+      raise ValueError("element type %s (bfloat16, float16 and float32 are built)" % like.dtype)
+    self.channels = c = like.shape[-1]
+    self.rows = like.numel() // c
+    if norm not in ("rms", "layer"):
+      raise ValueError("norm is 'rms' or 'layer', not %r" % (norm,))
+    self.layer = norm == "layer"
+    if not eps > 0:
+      raise ValueError("eps has to be positive")
+    if gate_act not in ("none", "sigmoid"):
+      raise ValueError("gate_act is 'none' or 'sigmoid', not %r" % (gate_act,))
+    self.sigmoid = gate_act == "sigmoid"
+    if y is None and (post_gamma is not None or gate is not None):
+      raise ValueError("post_gamma and gate belong to y")
+    if (post_beta is not None and post_gamma is None) or (pre_beta is not None and pre_gamma is None):
+      raise ValueError("a beta goes with its gamma")
+    if not self.layer and (post_beta is not None or pre_beta is not None):
+      raise ValueError("norm='rms' has no beta")
+    for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma),
+                    ("pre_beta", pre_beta)):
+      if t is not None and (t.shape != (c,) or t.dtype != torch.float32 or t.device != like.device
+                            or not t.is_contiguous()):
+        raise ValueError("%s: %d contiguous float32 values on %s" % (name, c, like.device))
+    self.group_rows, self.gate_pitch = 0, c
+    if gate is not None:
+      if gate.dtype == like.dtype and gate.shape == like.shape:
+        self.gate_pitch = _pitch("gate", gate, like)
+      elif gate.dtype == torch.float32 and gate.device == like.device and gate.dim() in (1, 2) and gate.shape[-1] == c:
+        groups = gate.numel() // c
+        if groups < 1 or self.rows % groups:
+          raise ValueError("gate: %d rows of it do not divide %d rows" % (groups, self.rows))
+        self.group_rows = self.rows // groups
+        self.gate_pitch = _row_pitch("gate", gate)
+      else:
+        raise ValueError("gate: one value per element in the rows' type, or float32 [groups, %d] with groups that "
+                         "divide the rows; got %s %s on %s" % (c, tuple(gate.shape), gate.dtype, gate.device))
+
+
+def _no_graph(**tensors):
+  """These entry points compute values; a gradient that autograd would have to record is refused, not lost."""
+  if torch.is_grad_enabled():
+    for name, t in tensors.items():
+      if t is not None and t.requires_grad:
+        raise ValueError("%s requires a gradient: it is computed by residual_norm_grad, call under torch.no_grad()"
+                         % name)
+
+
+def _normalised(v: torch.Tensor, layer: bool, eps: float):
+  if layer:
+    v = v - v.mean(-1, keepdim=True)
+  r = torch.rsqrt((v * v).mean(-1, keepdim=True) + eps)
+  return v * r, r
+
+
+def _normalised_grad(d, hat, r, layer):
+  d_mean = d.mean(-1, keepdim=True) if layer else 0.0
+  return r * (d - d_mean - hat * (d * hat).mean(-1, keepdim=True))
+
+
+def _gate_factor(s: _Seam, gate):
+  """The gate's factor per row and its derivative, in float32."""
+  g = gate.float().reshape(-1, s.channels)
+  g = g.repeat_interleave(s.group_rows, 0) if s.group_rows else g[:s.rows]
+  if not s.sigmoid:
+    return g, 1.0
+  a = torch.sigmoid(g)
+  return a, a * (1 - a)
+
+
+def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_gamma=None, post_beta=None, gate=None,
+                  gate_act: str = "none", residual_scale: float = 1.0, pre_gamma=None, pre_beta=None,
+                  norm: str = "rms", eps: float = 1e-6):
+  """What lies between two residual blocks, in one pass over the rows.
+
+      n = N(y) * post_gamma + post_beta             the norm after the block (n = y without post_gamma)
+      h = x + residual_scale * act(gate) * n        the residual stream (h is x without y)
+      z = N(h) * pre_gamma + pre_beta               the norm before the next block (None without pre_gamma)
+
+  returns (h, z).  `x`, `y` and the results are [..., channels] in bfloat16, float16 or float32, 1 to 8192
+  channels (pixels of an NHWC activation, tokens); rows may lie at any one distance, their channels next to each other.
+  N is v / sqrt(mean(v^2) + eps) with norm="rms", (v - mean) / sqrt(var + eps) with norm="layer".  gammas and
+  betas are float32 [channels], betas only with "layer".  `gate` is a value per element in the type of x, or float32
+  [groups, channels] (or [channels]) whose rows hold for rows / groups consecutive rows each: a learnt scale per channel,
+  a gate per image.  gate_act is "none" or "sigmoid".  Arithmetic is float32, z comes from the unrounded h.  Squares
+  are summed in float32: a row whose values pass 1e18 overflows there.
+  No graph is recorded; `residual_norm_grad` is the gradient.
+  """
+  s = _Seam(x, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps)
+  _no_graph(x=x, y=y, post_gamma=post_gamma, post_beta=post_beta, gate=gate, pre_gamma=pre_gamma, pre_beta=pre_beta)
+  pitch = dict(x=_row_pitch("x", x), gate=s.gate_pitch)
+  if y is not None:
+    pitch["y"] = _pitch("y", y, x)
+  if x.device.type == "cuda":
+    if s.channels > MAX_CHANNELS:
+      raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, s.channels))
+    from . import native  # pylint: disable=import-outside-toplevel
+    return native.residual_norm(x, y, s.rows, s.channels, pitch, gate, s.group_rows, s.sigmoid, s.layer,
+                                float(residual_scale), float(eps), post_gamma, post_beta, pre_gamma, pre_beta)
+  h, z = x.float().reshape(-1, s.channels), None
+  out = x
+  if y is not None:
+    n = y.float().reshape(-1, s.channels)
+    if post_gamma is not None:
+      n = _normalised(n, s.layer, eps)[0] * post_gamma
+      n = n if post_beta is None else n + post_beta
+    if gate is not None:
+      n = n * _gate_factor(s, gate)[0]
+    h = h + residual_scale * n
+    out = h.to(x.dtype).view(x.shape)
+  if pre_gamma is not None:
+    z = _normalised(h, s.layer, eps)[0] * pre_gamma
+    z = (z if pre_beta is None else z + pre_beta).to(x.dtype).view(x.shape)
+  return out, z
+
+
+def residual_norm_grad(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], h: torch.Tensor,
+                       y: Optional[torch.Tensor] = None, *, post_gamma=None, post_beta=None, gate=None,
+                       gate_act: str = "none", residual_scale: float = 1.0, pre_gamma=None, pre_beta=None,
+                       norm: str = "rms", eps: float = 1e-6) -> Dict[str, Optional[torch.Tensor]]:
+  """Gradient of `residual_norm` at its result h and its input y (x is not needed).
+
+  `dh`: gradient of h from its other uses (None: there are none), `dz`: gradient of z (given exactly when pre_gamma
+  is).  Returns a dict of dx, dy (the type of h), dgate (the type and shape of gate; a row of a [groups, channels] gate sums
+  over its rows), dpost_gamma, dpost_beta, dpre_gamma, dpre_beta (float32 [channels]), None for what was not
+  given.  The norms' statistics are taken from h and y again, so nothing has to be kept from the forward call.
+  Sums over rows are float32 in a fixed order: the same call gives the same bits.
+  """
+  s = _Seam(h, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps)
+  _no_graph(dh=dh, dz=dz, h=h, y=y, post_gamma=post_gamma, post_beta=post_beta, gate=gate, pre_gamma=pre_gamma,
+            pre_beta=pre_beta)
+  if (dz is None) != (pre_gamma is None):
+    raise ValueError("dz goes with pre_gamma")
+  if dz is None and dh is None:
+    raise ValueError("neither dh nor dz")
+  pitch = dict(h=_row_pitch("h", h), gate=s.gate_pitch)
+  for name, t in (("dh", dh), ("dz", dz), ("y", y)):
+    if t is not None:
+      pitch[name] = _pitch(name, t, h)
+  if h.device.type == "cuda":
+    if s.channels > MAX_CHANNELS:
+      raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, s.channels))
+    from . import native  # pylint: disable=import-outside-toplevel
+    return native.residual_norm_grad(dh, dz, h, y, s.rows, s.channels, pitch, gate, s.group_rows, s.sigmoid, s.layer,
+                                     float(residual_scale), float(eps), post_gamma, post_beta, pre_gamma, pre_beta)
+  c = s.channels
+  out: Dict[str, Optional[torch.Tensor]] = dict.fromkeys(
+      ("dx", "dy", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"))
+  up = dh.float().reshape(-1, c) if dh is not None else torch.zeros(s.rows, c)
+  if dz is not None:
+    d = dz.float().reshape(-1, c)
+    hat, r = _normalised(h.float().reshape(-1, c), s.layer, eps)
+    out["dpre_gamma"] = (d * hat).sum(0)
+    if pre_beta is not None:
+      out["dpre_beta"] = d.sum(0)
+    up = up + _normalised_grad(d * pre_gamma, hat, r, s.layer)
+  out["dx"] = up.to(h.dtype).view(h.shape)
+  if y is None:
+    return out
+  up = residual_scale * up
+  n = y.float().reshape(-1, c)
+  if post_gamma is not None:
+    hat, r = _normalised(n, s.layer, eps)
+    n = hat * post_gamma
+    n = n if post_beta is None else n + post_beta
+  if gate is not None:
+    a, slope = _gate_factor(s, gate)
+    dg = up * n * slope
+    if s.group_rows or not s.rows:
+      dg = dg.view(gate.numel() // c, -1, c).sum(1) if s.rows else torch.zeros(gate.shape)
+    out["dgate"] = dg.to(gate.dtype).view(gate.shape)
+    up = up * a
+  if post_gamma is not None:
+    out["dpost_gamma"] = (up * hat).sum(0)
+    if post_beta is not None:
+      out["dpost_beta"] = up.sum(0)
+    up = _normalised_grad(up * post_gamma, hat, r, s.layer)
+  out["dy"] = up.to(h.dtype).view(h.shape)
+  return out
+
+
+# ---- the norm over all gradients -------------------------------------------------------------------
+
+def _overlaps(spans) -> bool:
+  spans = sorted(s for s in spans if s[0] != s[1])
+  return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
+def _span(t: torch.Tensor):
+  return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+
+class TensorTable:
+  """A list of tensors as `global_norm` and `clip_by_global_norm` walk it, built once for gradients that live in the
+  same buffers step after step (a plan, like the launch plan of a training step).
+
+  `out`: where clipped tensors go, a list of the same shapes and types (the tensors themselves: in place); without
+  it they are clipped in place.  The table keeps the tensors alive and follows them: one whose storage was exchanged
+  since is looked up again by the next call.  Contiguous bfloat16, float16 or float32 tensors of one device; outputs may
+  not overlap each other, nor any input but their own.
+  """
+
+  def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
+    self.tensors = list(tensors)
+    self.out = self.tensors if out is None else list(out)
+    if not self.tensors:
+      raise ValueError("an empty list of tensors")
+    if len(self.out) != len(self.tensors):
+      raise ValueError("%d outputs for %d tensors" % (len(self.out), len(self.tensors)))
+    self.device = self.tensors[0].device
+    self._build()
+
+  def _build(self):
+    for i, (t, o) in enumerate(zip(self.tensors, self.out)):
+      if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("tensor %d: element type %s (bfloat16, float16 and float32 are built)" % (i, t.dtype))
+      if t.device != self.device or o.device != self.device:
+        raise ValueError("tensor %d: the list lives on %s" % (i, self.device))
+      if not t.is_contiguous() or not o.is_contiguous():
+        raise ValueError("tensor %d is not contiguous" % i)
+      if o.shape != t.shape or o.dtype != t.dtype:
+        raise ValueError("output %d: %s %s for %s %s" % (i, tuple(o.shape), o.dtype, tuple(t.shape), t.dtype))
+    self._at = [t.data_ptr() for t in self.tensors]
+    self._to = self._at if self.out is self.tensors else [o.data_ptr() for o in self.out]
+    # refused by clip_by_global_norm alone: a norm may count a tensor twice
+    outs = [_span(o) for o in self.out]
+    apart = [_span(t) for t, o in zip(self.tensors, self.out) if t.data_ptr() != o.data_ptr()]
+    self._clash = _overlaps(outs) or (bool(apart) and _overlaps_two(outs, apart))
+    self._list = None
+    if self.device.type == "cuda":
+      from . import native  # pylint: disable=import-outside-toplevel
+      self._list = native.ext().ClipList(self._at, self._to, [t.numel() for t in self.tensors],
+                                         [native.dtype_code(t.dtype) for t in self.tensors])
+
+  def _current(self) -> "TensorTable":
+    if self._at != list(map(torch.Tensor.data_ptr, self.tensors)) or (
+        self.out is not self.tensors and self._to != list(map(torch.Tensor.data_ptr, self.out))):
+      self._build()
+    return self
+
+
+def _overlaps_two(a, b) -> bool:
+  """Whether a span of `a` overlaps one of `b` (the spans of each list apart from one another, or not)."""
+  events = sorted([(s[0], s[1], 0) for s in a if s[0] != s[1]] + [(s[0], s[1], 1) for s in b if s[0] != s[1]])
+  ends = [0, 0]
+  for lo, hi, which in events:
+    if ends[1 - which] > lo:
+      return True
+    ends[which] = max(ends[which], hi)
+  return False
+
+
+def _table(tensors) -> TensorTable:
+  if isinstance(tensors, TensorTable):
+    return tensors._current()
+  if isinstance(tensors, torch.Tensor):
+    raise ValueError("a list of tensors (or a TensorTable), not a tensor")
+  return TensorTable(tensors)
+
+
+def _squares(tensors) -> torch.Tensor:
+  return torch.stack([t.detach().double().square().sum() for t in tensors]).sum()
+
+
+def global_norm(tensors) -> torch.Tensor:
+  """sqrt of the sum of squares over all tensors of a list or `TensorTable`: a float32 scalar on their device.
+
+  Squares are summed in 64 bits in a fixed order; nothing is read back to the host.
+  """
+  t = _table(tensors)
+  if t.device.type != "cuda":
+    return _squares(t.tensors).sqrt().float()
+  from . import native  # pylint: disable=import-outside-toplevel
+  return native.clip_list_norm(t)
+
+
+def clip_by_global_norm(tensors, clip_norm: float, use_norm: Optional[torch.Tensor] = None, out=None):
+  """Scales all tensors by min(1, clip_norm / norm) of their global norm, as tf.clip_by_global_norm does; returns
+  (list of clipped tensors, norm).
+
+  `tensors`: a list, clipped into new tensors or into `out` (a list of the same shapes and types; the list itself:
+  in place), or a `TensorTable`, which brings its own.  `use_norm`: a float32 scalar on the device that takes the
+  place of the norm (of a model whose gradients are spread over processes).  A norm that is infinite or NaN makes
+  every result NaN; a norm of zero changes nothing.  Nothing is read back to the host.
+  """
+  clip_norm = float(clip_norm)
+  if not clip_norm > 0:
+    raise ValueError("clip_norm has to be positive, got %r" % clip_norm)
+  if isinstance(tensors, TensorTable):
+    if out is not None:
+      raise ValueError("a TensorTable brings its own outputs")
+    t = tensors._current()
+  else:
+    tensors = list(tensors)
+    t = TensorTable(tensors, [torch.empty_like(x, memory_format=torch.contiguous_format) for x in tensors]
+                    if out is None else out)
+  if t._clash:
+    raise ValueError("outputs overlap each other, or another tensor's input")
+  if use_norm is not None and (use_norm.dtype != torch.float32 or use_norm.numel() != 1
+                               or use_norm.device != t.device):
+    raise ValueError("use_norm: a float32 scalar on %s" % t.device)
+  if t.device.type == "cuda":
+    from . import native  # pylint: disable=import-outside-toplevel
+    return list(t.out), native.clip_list_scale(t, clip_norm, use_norm)
+  with torch.no_grad():
+    norm = _squares(t.tensors).sqrt() if use_norm is None else use_norm.double().reshape(())
+    factor = torch.clamp(clip_norm / norm, max=1.0) if bool(torch.isfinite(norm)) else norm * float("nan")
+    for x, o in zip(t.tensors, t.out):
+      o.copy_(x.float() * factor.float())
+  return list(t.out), norm.float() if use_norm is None else use_norm
+
+
+def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity: torch.Tensor, l2x2: torch.Tensor,
+                            lr: float, momentum: float, clip_norm: float, grad_scale: float = 1.0,
+                            skip=None) -> torch.Tensor:
+  """`sgd_momentum_l2` with the gradient clipped to `clip_norm` by its global norm, in place; returns that norm (a
+  float32 scalar on the device, before clipping).
+
+      g  = grads * grad_scale + l2x2 * params
+      g <- g * min(1, clip_norm / |g|)
+      v <- momentum * v - lr * g
+      w <- w + v
+
+  The norm is that of the whole gradient, the regulariser's part included.  `skip` as in `sgd_momentum_l2`: with a
+  flag that is set nothing is updated.  A norm that is not finite, without `skip`, makes parameters and velocity NaN.
+  """
+  n = params.numel()
+  for name, t in (("params", params), ("grads", grads), ("velocity", velocity), ("l2x2", l2x2)):
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.device != params.device:
+      raise ValueError("clipped_sgd_momentum_l2 wants contiguous fp32 tensors on one device (%s)" % name)
+    if t.numel() != n and (name != "velocity" or momentum):
+      raise ValueError("clipped_sgd_momentum_l2: buffer sizes differ")
+  if n == 0:
+    raise ValueError("clipped_sgd_momentum_l2: no parameters")
+  if not clip_norm > 0:
+    raise ValueError("clip_norm has to be positive, got %r" % clip_norm)
+  spans = [_span(params), _span(grads), _span(l2x2)] + ([_span(velocity)] if momentum else [])
+  if _overlaps(spans):
+    raise ValueError("clipped_sgd_momentum_l2: buffers overlap")
+  if skip is not None and (skip.dtype != torch.float32 or skip.numel() < 2 or skip.device != params.device
+                           or not skip.is_contiguous()):
+    raise ValueError("skip: two contiguous float32 values on %s" % params.device)
+  if params.device.type == "cuda":
+    from . import native  # pylint: disable=import-outside-toplevel
+    return native.clipped_sgd_momentum_l2(params, grads, velocity, l2x2, lr, momentum, clip_norm, grad_scale, skip)
+  if skip is not None:
+    raise ValueError("a device-side skip flag needs the native optimizer kernel")
+  with torch.no_grad():
+    g = torch.addcmul(grads * grad_scale, l2x2, params)
+    norm = g.double().square().sum().sqrt()
+    factor = float(torch.clamp(clip_norm / norm, max=1.0)) if bool(torch.isfinite(norm)) else float("nan")
+    if momentum:
+      velocity.mul_(momentum).add_(g, alpha=-lr * factor)
+      params.add_(velocity)
+    else:
+      params.add_(g, alpha=-lr * factor)
+  return norm.float()

@@ -118,6 +118,13 @@ class Model:
     del run_eagerly, experimental_run_tf_function   # accepted for call-site parity
     if loss not in SUPPORTED_LOSSES:
       raise ValueError("loss must be one of %s" % (SUPPORTED_LOSSES,))
+    if self.strategy is not None and not self.strategy.synchronous:
+      opt = optimizer
+      while opt is not None:
+        if getattr(opt, "global_clipnorm", None) is not None:
+          raise ValueError("global_clipnorm: an asynchronous parameter server updates its shards without the norm "
+                           "over all variables")
+        opt = getattr(opt, "inner", None)
     self.optimizer = optimizer
     self.loss = loss
     self._acc_name = None

@@ -67,16 +67,24 @@ class Optimizer:
 
 
 class SGD(Optimizer):
-  """Keras-form SGD with (non-Nesterov) momentum and fused L2."""
+  """Keras-form SGD with (non-Nesterov) momentum and fused L2.
+
+  `global_clipnorm` (Keras' argument of that name): the gradient of the step - averaged over the replicas, unscaled,
+  the L2 term included - is scaled down to that norm where its norm over all variables is larger.  Norm and factor
+  stay on the device; `gradient_norm` holds the last step's norm (a scalar tensor, before clipping)."""
 
   slot_names = ("momentum",)
 
   def __init__(self, learning_rate: Schedule = 0.01, momentum: float = 0.0,
-               nesterov: bool = False):
+               nesterov: bool = False, global_clipnorm: Optional[float] = None):
     super().__init__(learning_rate)
     if nesterov:
       raise NotImplementedError("the reference uses plain momentum")
+    if global_clipnorm is not None and not global_clipnorm > 0:
+      raise ValueError("global_clipnorm has to be positive, got %r" % (global_clipnorm,))
     self.momentum = float(momentum)
+    self.global_clipnorm = None if global_clipnorm is None else float(global_clipnorm)
+    self.gradient_norm: Optional[torch.Tensor] = None
 
   def apply_gradients(self, store: ParamStore, grad_divisor: float = 1.0,
                       executor=None, skip=None) -> bool:
@@ -85,8 +93,13 @@ class SGD(Optimizer):
     lr = self.current_lr()
     from ..ops import fused  # pylint: disable=import-outside-toplevel
     v = store.slot("momentum") if self.momentum else store.params  # unused when momentum == 0
-    fused.sgd_momentum_l2(store.params, store.grads, v, store.l2_vector(), lr,
-                          self.momentum, 1.0 / grad_divisor, skip)
+    if self.global_clipnorm is not None:
+      self.gradient_norm = fused.clipped_sgd_momentum_l2(
+          store.params, store.grads, v, store.l2_vector(), lr, self.momentum, self.global_clipnorm,
+          1.0 / grad_divisor, skip)
+    else:
+      fused.sgd_momentum_l2(store.params, store.grads, v, store.l2_vector(), lr,
+                            self.momentum, 1.0 / grad_divisor, skip)
     store.version += 1
     if executor is not None:
       executor.params_updated()
@@ -96,6 +109,8 @@ class SGD(Optimizer):
   def get_config(self):
     c = super().get_config()
     c.update(momentum=self.momentum, nesterov=False)
+    if self.global_clipnorm is not None:
+      c.update(global_clipnorm=self.global_clipnorm)
     return c
 
 
