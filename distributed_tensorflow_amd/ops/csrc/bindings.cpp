@@ -165,19 +165,29 @@ WgradParams wgrad_from_dict(const py::dict& d) {
   return p;
 }
 
-ResidualNormParams residual_norm_from_dict(const py::dict& d, bool backward) {
+ResidualNormParams residual_norm_of(int dt, int P, int C, int layer, int sigmoid, float scale, float eps, uintptr_t y,
+                                    int64_t ldy, uintptr_t gate, int64_t ldgate, int group_rows, uintptr_t post_gamma,
+                                    uintptr_t post_beta, uintptr_t pre_gamma, uintptr_t pre_beta) {
   ResidualNormParams p;
-  p.dt = get_or<int>(d, "dt", DT_BF16);
-  p.P = get<int>(d, "P"); p.C = get<int>(d, "C");
-  p.layer = get_or<int>(d, "layer", 0); p.sigmoid = get_or<int>(d, "sigmoid", 0);
-  p.scale = get_or<float>(d, "scale", 1.f); p.eps = get_or<float>(d, "eps", 1e-6f);
-  p.y = ptr<const void>(d, "y", false); p.ldy = get_or<int64_t>(d, "ldy", p.C);
-  p.gate = ptr<const void>(d, "gate", false); p.ldgate = get_or<int64_t>(d, "ldgate", p.C);
+  p.dt = dt; p.P = P; p.C = C; p.layer = layer; p.sigmoid = sigmoid; p.scale = scale; p.eps = eps;
+  p.y = reinterpret_cast<const void*>(y); p.ldy = ldy;
+  p.gate = reinterpret_cast<const void*>(gate); p.ldgate = ldgate;
   // a gate row per `group_rows` rows (fp32), or 0: one per row in the rows' own type
-  p.group_rows = get_or<int>(d, "group_rows", 0);
-  p.gate_mode = !p.gate ? GATE_NONE : p.group_rows > 0 ? GATE_GROUP : GATE_ELEMENT;
-  p.post_gamma = ptr<const float>(d, "post_gamma", false); p.post_beta = ptr<const float>(d, "post_beta", false);
-  p.pre_gamma = ptr<const float>(d, "pre_gamma", false); p.pre_beta = ptr<const float>(d, "pre_beta", false);
+  p.group_rows = group_rows;
+  p.gate_mode = !gate ? GATE_NONE : group_rows > 0 ? GATE_GROUP : GATE_ELEMENT;
+  p.post_gamma = reinterpret_cast<const float*>(post_gamma); p.post_beta = reinterpret_cast<const float*>(post_beta);
+  p.pre_gamma = reinterpret_cast<const float*>(pre_gamma); p.pre_beta = reinterpret_cast<const float*>(pre_beta);
+  return p;
+}
+
+ResidualNormParams residual_norm_from_dict(const py::dict& d, bool backward) {
+  const int C = get<int>(d, "C");
+  ResidualNormParams p = residual_norm_of(
+      get_or<int>(d, "dt", DT_BF16), get<int>(d, "P"), C, get_or<int>(d, "layer", 0), get_or<int>(d, "sigmoid", 0),
+      get_or<float>(d, "scale", 1.f), get_or<float>(d, "eps", 1e-6f), get_or<uintptr_t>(d, "y", 0),
+      get_or<int64_t>(d, "ldy", C), get_or<uintptr_t>(d, "gate", 0), get_or<int64_t>(d, "ldgate", C),
+      get_or<int>(d, "group_rows", 0), get_or<uintptr_t>(d, "post_gamma", 0), get_or<uintptr_t>(d, "post_beta", 0),
+      get_or<uintptr_t>(d, "pre_gamma", 0), get_or<uintptr_t>(d, "pre_beta", 0));
   if (!backward) {
     p.x = ptr<const void>(d, "x"); p.ldx = get_or<int64_t>(d, "ldx", p.C);
     p.h = ptr<void>(d, "h", p.y != nullptr); p.z = ptr<void>(d, "z", p.pre_gamma != nullptr);
@@ -394,15 +404,6 @@ Launch make_op(const std::string& kind, const py::dict& d, bool planned = false)
     auto skip = ptr<const float>(d, "skip", false);     // device [skip flag, inverse loss scale]
     const int um = get_or<int>(d, "use_momentum", mom != 0.f ? 1 : 0);
     return [=](hipStream_t s) { launch_sgd_momentum_l2(p, g, v, l2, n, lr, mom, gs, um, hyper, skip, s); };
-  }
-  if (kind == "clipped_sgd") {
-    auto p = ptr<float>(d, "p"); auto g = ptr<const float>(d, "g"); auto v = ptr<float>(d, "v");
-    auto l2 = ptr<const float>(d, "l2x2"); auto skip = ptr<const float>(d, "skip", false);
-    auto ws = ptr<double>(d, "ws"); auto norm = ptr<float>(d, "norm", false);    // clipped_sgd_blocks(n) doubles
-    const size_t n = get<size_t>(d, "n");
-    const float lr = get<float>(d, "lr"), mom = get<float>(d, "momentum"), clip = get<float>(d, "clip");
-    const float gs = get_or<float>(d, "grad_scale", 1.f);
-    return [=](hipStream_t s) { launch_clipped_sgd_momentum_l2(p, g, v, l2, n, lr, mom, gs, clip, skip, ws, norm, s); };
   }
   if (kind == "residual_norm_fwd" || kind == "residual_norm_bwd") {
     const bool backward = kind == "residual_norm_bwd";
@@ -807,13 +808,56 @@ PYBIND11_MODULE(_dtf_native, m) {
   m.def("bn_workspace_floats", []() { return bn_workspace_floats(); });
   m.def("bn_tail_floats", []() { return bn_tail_floats(); });
   m.def("bn_fold_desc_size", []() { return bn_fold_desc_size(); });
+  // The same launches as the plan entries residual_norm_fwd / _bwd, with plain arguments: a dict of twenty entries costs
+  // more host time than the kernel of a short call (5 of 18 us for one row).
+  m.def("residual_norm_fwd", [](int dt, int P, int C, int layer, int sigmoid, float scale, float eps, uintptr_t x,
+                                int64_t ldx, uintptr_t y, int64_t ldy, uintptr_t gate, int64_t ldgate, int group_rows,
+                                uintptr_t post_gamma, uintptr_t post_beta, uintptr_t pre_gamma, uintptr_t pre_beta,
+                                uintptr_t h, uintptr_t z, uintptr_t stream) {
+    ResidualNormParams p = residual_norm_of(dt, P, C, layer, sigmoid, scale, eps, y, ldy, gate, ldgate, group_rows,
+                                            post_gamma, post_beta, pre_gamma, pre_beta);
+    p.x = reinterpret_cast<const void*>(x); p.ldx = ldx;
+    p.h = reinterpret_cast<void*>(h); p.z = reinterpret_cast<void*>(z);
+    launch_residual_norm_fwd(p, reinterpret_cast<hipStream_t>(stream));
+    check_launch();
+  });
+  m.def("residual_norm_bwd", [](int dt, int P, int C, int layer, int sigmoid, float scale, float eps, uintptr_t h,
+                                int64_t ldh, uintptr_t y, int64_t ldy, uintptr_t gate, int64_t ldgate, int group_rows,
+                                uintptr_t post_gamma, uintptr_t post_beta, uintptr_t pre_gamma, uintptr_t pre_beta,
+                                uintptr_t dh, int64_t lddh, uintptr_t dz, int64_t lddz, uintptr_t dx, uintptr_t dy,
+                                uintptr_t dgate, uintptr_t vectors, uintptr_t ws, uintptr_t stream) {
+    ResidualNormParams p = residual_norm_of(dt, P, C, layer, sigmoid, scale, eps, y, ldy, gate, ldgate, group_rows,
+                                            post_gamma, post_beta, pre_gamma, pre_beta);
+    p.x = reinterpret_cast<const void*>(h); p.ldx = ldh;
+    p.dh = reinterpret_cast<const void*>(dh); p.lddh = lddh;
+    p.dz = reinterpret_cast<const void*>(dz); p.lddz = lddz;
+    p.dx = reinterpret_cast<void*>(dx); p.dy = reinterpret_cast<void*>(dy);
+    p.dgate = reinterpret_cast<void*>(dgate);
+    p.ws = reinterpret_cast<float*>(ws);
+    float* v = reinterpret_cast<float*>(vectors);      // [those that are there][C]
+    if (pre_gamma) { p.dpre_gamma = v; v += C; }
+    if (pre_beta) { p.dpre_beta = v; v += C; }
+    if (post_gamma) { p.dpost_gamma = v; v += C; }
+    if (post_beta) p.dpost_beta = v;
+    launch_residual_norm_bwd(p, reinterpret_cast<hipStream_t>(stream));
+    check_launch();
+  });
   m.def("residual_norm_workspace_floats", [](int P, int C, int group_rows) {
     ResidualNormParams p;
     p.P = P; p.C = C; p.group_rows = group_rows;
     p.gate_mode = group_rows > 0 ? GATE_GROUP : GATE_NONE;
     return residual_norm_workspace_floats(p);
   }, "Floats that residual_norm_bwd keeps its partial sums in; group_rows: rows that share a gate row, or 0");
-  m.def("clipped_sgd_blocks", &clipped_sgd_blocks);
+  m.def("clipped_sgd_blocks", &clipped_sgd_blocks, "Doubles of workspace for an update of that many elements");
+  m.def("clipped_sgd", [](uintptr_t p, uintptr_t g, uintptr_t v, uintptr_t l2x2, size_t n, float lr, float momentum,
+                          float grad_scale, float clip, uintptr_t skip, uintptr_t ws, uintptr_t norm, uintptr_t s) {
+    launch_clipped_sgd_momentum_l2(reinterpret_cast<float*>(p), reinterpret_cast<const float*>(g),
+                                   reinterpret_cast<float*>(v), reinterpret_cast<const float*>(l2x2), n, lr, momentum,
+                                   grad_scale, clip, reinterpret_cast<const float*>(skip),
+                                   reinterpret_cast<double*>(ws), reinterpret_cast<float*>(norm),
+                                   reinterpret_cast<hipStream_t>(s));
+    check_launch();
+  });
   m.attr("RESIDUAL_NORM_MAX_C") = RESIDUAL_NORM_MAX_C;
   py::class_<ClipList>(m, "ClipList")
       .def(py::init([](const std::vector<uintptr_t>& in, const std::vector<uintptr_t>& out,

@@ -24,22 +24,36 @@ namespace {
 struct __attribute__((packed, aligned(2))) Any16 { u32x4 v; };
 struct __attribute__((packed, aligned(4))) Any16F { f32x4 v; };
 
-// Eight channels from `c` on of the row at `p`, as floats; what lies past channel C - 1 is zero.
+// Eight channels from `c` on of the row at `p`, as they sit in memory; what lies past channel C - 1 is zero.
 template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, int c, int C, float* f) {
+__device__ __forceinline__ Raw8<DT> load_raw(const typename Elem<DT>::T* p, int c, int C) {
+  Raw8<DT> r = zero_raw<DT>();
   if (c + 8 <= C) {
-    Raw8<DT> r;
     if constexpr (DT == DT_F32) {
       r.lo = reinterpret_cast<const Any16F*>(p + c)->v;
       r.hi = reinterpret_cast<const Any16F*>(p + c + 4)->v;
     } else {
       r.v = reinterpret_cast<const Any16*>(p + c)->v;
     }
-    unpack8<DT>(r, f);
-  } else {
+  } else if (c < C) {
+    if constexpr (DT == DT_F32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = c + j < C ? to_f<DT>(p[c + j]) : 0.f;
+      for (int j = 0; j < 4; ++j) {
+        if (c + j < C) r.lo[j] = p[c + j];
+        if (c + 4 + j < C) r.hi[j] = p[c + 4 + j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < C) r.v[j >> 1] |= (uint32_t)p[c + j] << (16 * (j & 1));
+    }
   }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, int c, int C, float* f) {
+  unpack8<DT>(load_raw<DT>(p, c, C), f);
 }
 
 template <int DT>
@@ -69,15 +83,39 @@ __device__ __forceinline__ float sigmoid_f(float g) {
   else return __builtin_amdgcn_rcpf(1.f + __expf(-g));
 }
 
+// v + v of the lane that is `O` away, in every lane (O = 1, 2, 4 .. 32 in this order: from O = 4 on the lanes of the
+// smaller groups hold the same value already, so a mirrored row does for an exchange).  Register to register: no trip
+// through LDS.
+template <int O>
+__device__ __forceinline__ float add_lane(float v) {
+  const int i = __float_as_int(v);
+  if constexpr (O == 1) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0xB1, 0xf, 0xf, true));
+  else if constexpr (O == 2) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x4E, 0xf, 0xf, true));
+  else if constexpr (O == 4) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x141, 0xf, 0xf, true));
+  else if constexpr (O == 8) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x140, 0xf, 0xf, true));
+  else if constexpr (O == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(i, i, false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+  }
+}
+
 // Sums of N values over the lanes of a row, given to all of them.  LPR lanes of a wave hold a narrow row; a wide one
 // has `waves` whole waves, joined through the half `turn & 1` of `red`: the barrier of the next sum separates this
 // sum's reads from the writes after next.
 template <int LPR, bool WIDE, int N>
 __device__ __forceinline__ void row_sums(float* v, float (*red)[4][8], int waves, int& turn) {
 #pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  for (int i = 0; i < N; ++i) {
+    v[i] = add_lane<1>(v[i]);
+    if constexpr (LPR >= 4) v[i] = add_lane<2>(v[i]);
+    if constexpr (LPR >= 8) v[i] = add_lane<4>(v[i]);
+    if constexpr (LPR >= 16) v[i] = add_lane<8>(v[i]);
+    if constexpr (LPR >= 32) v[i] = add_lane<16>(v[i]);
+    if constexpr (LPR >= 64) v[i] = add_lane<32>(v[i]);
+  }
   if constexpr (WIDE) {
     float (*mine)[8] = red[turn & 1];
     ++turn;
@@ -265,13 +303,37 @@ BwdPlan plan_bwd(const ResidualNormParams& p) {
 
 // Partial sums: [vector][block][C]; which vectors are kept goes by the gradients asked for.
 struct Partials {
-  float* row[5];      // dpre_gamma, dpre_beta, dpost_gamma, dpost_beta, dgate
+  float* row[5];      // dpre_gamma, dpost_gamma, dpre_beta, dpost_beta, dgate
 };
 
-template <int DT, int LPR, bool WIDE, int K>
+// The tensors of a row as they sit in memory.
+template <int DT, int K>
+struct RowIn {
+  Raw8<DT> dh[K], dz[K], h[K], y[K], gate[K];
+};
+
+template <int DT, int K>
+__device__ __forceinline__ void load_row(RowIn<DT, K>& in, const ResidualNormParams& p, int64_t r, const int* c, int C) {
+  typedef typename Elem<DT>::T T;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    in.dh[k] = zero_raw<DT>();
+    if (p.dh) in.dh[k] = load_raw<DT>(reinterpret_cast<const T*>(p.dh) + r * p.lddh, c[k], C);
+    if (p.dz) {
+      in.dz[k] = load_raw<DT>(reinterpret_cast<const T*>(p.dz) + r * p.lddz, c[k], C);
+      in.h[k] = load_raw<DT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], C);
+    }
+    if (p.y) in.y[k] = load_raw<DT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
+    if (p.gate_mode == GATE_ELEMENT) in.gate[k] = load_raw<DT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
+  }
+}
+
+template <int DT, int LPR, bool WIDE, int K, bool LAYER, bool GROUP>
 __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
                                                                const Partials part) {
   typedef typename Elem<DT>::T T;
+  // sums over rows: of the two gammas, with LAYER of the two betas, with GROUP of the gate
+  constexpr int SUMS = 2 + (LAYER ? 2 : 0) + (GROUP ? 1 : 0), GATE = SUMS - 1;
   __shared__ float red[2][4][8];
   __shared__ float join[WIDE ? 1 : 256 * 8];
   int turn = 0;
@@ -285,22 +347,20 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
   int c[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) c[k] = (lane + k * lanes) * 8;
-  float acc[5][K][8];
+  float acc[SUMS][K][8];
 #pragma unroll
-  for (int i = 0; i < 5; ++i)
+  for (int i = 0; i < SUMS; ++i)
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[i][k][j] = 0.f;
   float pw[K][8], pb[K][8], qw[K][8];     // post_gamma, post_beta, pre_gamma
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) pw[k][j] = pb[k][j] = qw[k][j] = 0.f;
-#pragma unroll
   for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { pw[k][j] = 1.f; pb[k][j] = qw[k][j] = 0.f; }
     if (p.post_gamma) load8<DT_F32>(p.post_gamma, c[k], C, pw[k]);
-    if (p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, pb[k]);
+    if (LAYER && p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, pb[k]);
     if (p.pre_gamma) load8<DT_F32>(p.pre_gamma, c[k], C, qw[k]);
   }
   // the sets of groups this block works on, and the rows of a group that are its own
@@ -315,160 +375,211 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
     const int group = plan.own_groups ? set * slots + slot : set;
     const bool group_live = group < plan.groups;
     float g[K][8];
-    if (p.gate_mode == GATE_GROUP) {
+    if constexpr (GROUP) {
       const float* row_g = reinterpret_cast<const float*>(p.gate) + (int64_t)(group_live ? group : 0) * p.ldgate;
 #pragma unroll
-      for (int k = 0; k < K; ++k) load8<DT_F32>(row_g, c[k], C, g[k]);
+      for (int k = 0; k < K; ++k) {
+        load8<DT_F32>(row_g, c[k], C, g[k]);
+        if (p.sigmoid) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
+        }
+      }
     }
-    for (int rr = row0; rr < row1; rr += step) {
+    // a row that is not there has no channels: zeros are read and nothing is written for it
+    auto row_of = [&](int rr, int64_t* r) {
       const int in_group = plan.own_groups ? rr : rr + slot;
       const bool live = group_live && in_group < row1;
-      const int Cr = live ? C : 0;
-      const int64_t r = live ? (int64_t)group * plan.group_rows + in_group : 0;
-      float up[K][8], dz[K][8], h[K][8], v[K][8], a[K][8], slope[K][8];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (p.dh) load8<DT>(reinterpret_cast<const T*>(p.dh) + r * p.lddh, c[k], Cr, up[k]);
-        if (p.dz) load8<DT>(reinterpret_cast<const T*>(p.dz) + r * p.lddz, c[k], Cr, dz[k]);
-        if (p.dz) load8<DT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], Cr, h[k]);
-        if (p.y) load8<DT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], Cr, v[k]);
+      *r = live ? (int64_t)group * plan.group_rows + in_group : 0;
+      return live ? C : 0;
+    };
+    RowIn<DT, K> next;
+    int64_t r_next = 0;
+    int C_next = 0;
+    if (row0 < row1) {
+      C_next = row_of(row0, &r_next);
+      load_row<DT, K>(next, p, r_next, c, C_next);
+    }
+    for (int rr = row0; rr < row1; rr += step) {
+      const RowIn<DT, K> in = next;
+      const int64_t r = r_next;
+      const int Cr = C_next;
+      if (rr + step < row1) {          // the next row's loads are under way while this row's sums are taken
+        C_next = row_of(rr + step, &r_next);
+        load_row<DT, K>(next, p, r_next, c, C_next);
       }
-      if (p.gate_mode == GATE_ELEMENT) {
+      float up[K][8], h[K][8], v[K][8];
 #pragma unroll
-        for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], Cr, a[k]);
+      for (int k = 0; k < K; ++k) unpack8<DT>(in.dh[k], up[k]);
+      float s[3] = {0.f, 0.f, 0.f};
+      float rs = 1.f, m_d = 0.f;
+      if (p.y) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) unpack8<DT>(in.y[k], v[k]);
       } else {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a[k][j] = p.gate_mode == GATE_GROUP ? g[k][j] : 1.f;
+          for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
       }
-      if (!p.dh) {
+      if (p.dz) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) unpack8<DT>(in.h[k], h[k]);
+      } else {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) up[k][j] = 0.f;
+          for (int j = 0; j < 8; ++j) h[k][j] = 0.f;
       }
+      if (p.dz || p.post_gamma) {
+        // both norms' statistics and what the first gradient needs come from the same sums
+        if constexpr (LAYER) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+          for (int k = 0; k < K; ++k) {
+            float dz[8];
+            if (p.dz) unpack8<DT>(in.dz[k], dz);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (p.sigmoid) {
-            a[k][j] = sigmoid_f<DT>(a[k][j]);
-            slope[k][j] = a[k][j] * (1.f - a[k][j]);
-          } else {
-            slope[k][j] = 1.f;
+            for (int j = 0; j < 8; ++j) {
+              s[0] += h[k][j];
+              s[1] += v[k][j];
+              if (p.dz) s[2] += dz[j] * qw[k][j];
+            }
+          }
+          row_sums<LPR, WIDE, 3>(s, red, waves, turn);
+          const float mean_h = s[0] * inv_c, mean_y = p.post_gamma ? s[1] * inv_c : 0.f;
+          m_d = s[2] * inv_c;
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              h[k][j] = c[k] + j < Cr ? h[k][j] - mean_h : 0.f;
+              v[k][j] = c[k] + j < Cr ? v[k][j] - mean_y : 0.f;
+            }
+          s[0] = s[1] = s[2] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float dz[8];
+          if (p.dz) unpack8<DT>(in.dz[k], dz);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            s[0] += h[k][j] * h[k][j];
+            s[1] += v[k][j] * v[k][j];
+            if (p.dz) s[2] += dz[j] * qw[k][j] * h[k][j];
           }
         }
+        row_sums<LPR, WIDE, 3>(s, red, waves, turn);
+        if (p.post_gamma) rs = 1.f / sqrtf(s[1] * inv_c + p.eps);
+      }
       if (p.dz) {
-        const float rs = normalise<LPR, WIDE, K>(h, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
-        float s[2] = {0.f, 0.f};
+        const float rh = 1.f / sqrtf(s[0] * inv_c + p.eps), m_dot = s[2] * rh * inv_c;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            h[k][j] *= rs;
-            const float d = dz[k][j] * qw[k][j];
-            s[0] += d * h[k][j];
-            s[1] += d;
-          }
-        row_sums<LPR, WIDE, 2>(s, red, waves, turn);
-        const float m_dot = s[0] * inv_c, m_d = p.layer ? s[1] * inv_c : 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+          float dz[8];
+          unpack8<DT>(in.dz[k], dz);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            up[k][j] += rs * (dz[k][j] * qw[k][j] - m_d - h[k][j] * m_dot);
-            acc[0][k][j] += dz[k][j] * h[k][j];
-            acc[1][k][j] += dz[k][j];
+            const float hat = h[k][j] * rh;
+            up[k][j] += rh * (dz[j] * qw[k][j] - m_d - hat * m_dot);
+            acc[0][k][j] += dz[j] * hat;
+            if constexpr (LAYER) acc[2][k][j] += dz[j];
           }
+        }
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) store8<DT>(reinterpret_cast<T*>(p.dx) + r * C, c[k], Cr, up[k]);
       if (!p.y) continue;
-      float rs = 1.f;
-      if (p.post_gamma) rs = normalise<LPR, WIDE, K>(v, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
-      float s[2] = {0.f, 0.f};
+      float t[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        float dg[8];
+        float a[8], dg[8];
+        if constexpr (!GROUP) {
+          if (p.gate_mode == GATE_ELEMENT) unpack8<DT>(in.gate[k], a);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          // a dead row or channel has h, dz, dh, y of zero; its `up` is not (the mean of dz' under `layer`)
+          // a dead row or channel has h, dz, dh, y of zero; its `up` is not (the mean of dz' under LAYER)
           const float u = c[k] + j < Cr ? p.scale * up[k][j] : 0.f;
           const float hat = v[k][j] * rs;
-          const float n = p.post_gamma ? hat * pw[k][j] + pb[k][j] : hat;
-          const float dn = u * a[k][j];
+          const float n = hat * pw[k][j] + pb[k][j];
+          float dn = u;
           dg[j] = u * n;
-          acc[4][k][j] += dg[j];
-          dg[j] *= slope[k][j];
-          acc[2][k][j] += dn * hat;
-          acc[3][k][j] += dn;
+          if constexpr (GROUP) {
+            dn *= g[k][j];
+            acc[GATE][k][j] += dg[j];
+          } else if (p.gate_mode == GATE_ELEMENT) {
+            if (p.sigmoid) {
+              a[j] = sigmoid_f<DT>(a[j]);
+              dg[j] *= a[j] * (1.f - a[j]);
+            }
+            dn *= a[j];
+          }
+          acc[1][k][j] += dn * hat;
+          if constexpr (LAYER) acc[3][k][j] += dn;
           v[k][j] = hat;
-          up[k][j] = p.post_gamma ? dn * pw[k][j] : dn;
-          s[0] += up[k][j] * hat;
-          s[1] += up[k][j];
+          up[k][j] = dn * pw[k][j];
+          t[0] += up[k][j] * hat;
+          t[1] += up[k][j];
         }
-        if (p.gate_mode == GATE_ELEMENT) store8<DT>(reinterpret_cast<T*>(p.dgate) + r * C, c[k], Cr, dg);
+        if constexpr (!GROUP) {
+          if (p.gate_mode == GATE_ELEMENT) store8<DT>(reinterpret_cast<T*>(p.dgate) + r * C, c[k], Cr, dg);
+        }
       }
       if (p.post_gamma) {
-        row_sums<LPR, WIDE, 2>(s, red, waves, turn);
-        const float m_dot = s[0] * inv_c, m_d = p.layer ? s[1] * inv_c : 0.f;
+        row_sums<LPR, WIDE, LAYER ? 2 : 1>(t, red, waves, turn);
+        const float m_dot = t[0] * inv_c, m_t = LAYER ? t[1] * inv_c : 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) up[k][j] = rs * (up[k][j] - m_d - v[k][j] * m_dot);
+          for (int j = 0; j < 8; ++j) up[k][j] = rs * (up[k][j] - m_t - v[k][j] * m_dot);
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) store8<DT>(reinterpret_cast<T*>(p.dy) + r * C, c[k], Cr, up[k]);
     }
-    if (p.gate_mode == GATE_GROUP && plan.parts == 1) {
+    if (GROUP && plan.parts == 1) {
       // whole groups: the gate's gradient is complete here
-      if (!WIDE && !plan.own_groups) {
-        static_assert(WIDE || K == 1, "narrow rows have one chunk a lane");
-        __syncthreads();
+      if constexpr (!WIDE) {
+        if (!plan.own_groups) {       // summed over the slots, lane by lane of slot 0
+          __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) join[slot * LPR * 8 + lane * 8 + j] = acc[4][0][j];
-        __syncthreads();
-        for (int col = threadIdx.x; col < C; col += 256) {
-          float sum = 0.f;
-          for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + col];
-          float f = 1.f;
-          if (p.sigmoid) {
-            const float sg = sigmoid_f<DT>(reinterpret_cast<const float*>(p.gate)[(int64_t)group * p.ldgate + col]);
-            f = sg * (1.f - sg);
+          for (int j = 0; j < 8; ++j) join[slot * LPR * 8 + lane * 8 + j] = acc[GATE][0][j];
+          __syncthreads();
+          if (slot == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {       // eight sums of `slots` values each, once a group
+              float sum = 0.f;
+#pragma unroll 4
+              for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + lane * 8 + j];
+              acc[GATE][0][j] = sum;
+            }
           }
-          reinterpret_cast<float*>(p.dgate)[(int64_t)group * C + col] = sum * f;
         }
-      } else if (group_live) {
+      }
+      if (group_live && (WIDE || plan.own_groups || slot == 0)) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          float dg[8];
+          if (p.sigmoid) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float f = 1.f;
-            if (p.sigmoid) {
-              const float sg = sigmoid_f<DT>(g[k][j]);
-              f = sg * (1.f - sg);
-            }
-            dg[j] = acc[4][k][j] * f;
+            for (int j = 0; j < 8; ++j) acc[GATE][k][j] *= g[k][j] * (1.f - g[k][j]);
           }
-          store8<DT_F32>(reinterpret_cast<float*>(p.dgate) + (int64_t)group * C, c[k], C, dg);
+          store8<DT_F32>(reinterpret_cast<float*>(p.dgate) + (int64_t)group * C, c[k], C, acc[GATE][k]);
         }
       }
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[4][k][j] = 0.f;
+        for (int j = 0; j < 8; ++j) acc[GATE][k][j] = 0.f;
     }
   }
   // the block's row of partial sums
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    if (!part.row[i]) continue;
-    float* out = part.row[i] + (int64_t)blockIdx.x * C;
+  for (int i = 0; i < SUMS; ++i) {
+    float* to = part.row[GROUP && i == GATE ? 4 : i];
+    if (!to) continue;
+    to += (int64_t)blockIdx.x * C;
     if constexpr (WIDE) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) store8<DT_F32>(out, c[k], C, acc[i][k]);
+      for (int k = 0; k < K; ++k) store8<DT_F32>(to, c[k], C, acc[i][k]);
     } else {
       __syncthreads();
 #pragma unroll
@@ -476,38 +587,71 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
       __syncthreads();
       for (int col = threadIdx.x; col < C; col += 256) {
         float sum = 0.f;
+#pragma unroll 8
         for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + col];
-        out[col] = sum;
+        to[col] = sum;
       }
     }
   }
 }
 
-// Sums the blocks' partial rows: vector blockIdx.y, 32 columns a block, 32 slices of the rows.  For the gate's
-// gradient (`of_group`, vector 4) the rows of one group are `parts` consecutive ones and blockIdx.z is the group.
+// Sums the blocks' partial rows, in one launch.  The vectors' rows (all blocks') and a gate's (of one group, `parts`
+// of them) are taken 32 columns a block in 32 slices; gates of few parts go a column a thread, 1024 a block, where
+// slices would leave most of a block idle (256 groups of 4 parts, 2048 columns: 35 us in slices, 5 us this way).
 struct Finish {
   const float* from[5];
   float* to[5];
   const float* gate;
   int64_t ldgate;
-  int C, rows, parts, sigmoid;
+  int C, rows, parts, groups, sigmoid;
+  int vector_blocks;      // blocks of the vectors; the gate's follow
 };
+constexpr int FEW_PARTS = 32;
 
 template <int DT>
-__global__ __launch_bounds__(1024) void finish_kernel(const Finish f, int first) {
+__global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
   __shared__ float join[32][33];
-  const int i = first + blockIdx.y;
-  const int rows = i == 4 ? f.parts : f.rows, group = blockIdx.z;
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  const int cols = (f.C + 31) / 32;
+  int b = (int)blockIdx.x, i = 4, group = 0, rows = f.parts, col;
+  if (b < f.vector_blocks) {
+    // the b / cols-th vector that is wanted
+    int skip = b / cols;
+    i = 0;
+    while (f.to[i] == nullptr || skip-- > 0) ++i;
+    b %= cols;
+    rows = f.rows;
+  } else {
+    b -= f.vector_blocks;
+    if (f.parts <= FEW_PARTS) {
+      const int wide_cols = (f.C + 1023) / 1024;
+      group = b / wide_cols;
+      col = (b % wide_cols) * 1024 + (int)threadIdx.x;
+      if (col >= f.C) return;
+      const float* from = f.from[4] + (int64_t)group * f.parts * f.C + col;
+      float sum = 0.f;
+#pragma unroll 4
+      for (int r = 0; r < f.parts; ++r) sum += from[(int64_t)r * f.C];
+      if (f.sigmoid) {
+        const float sg = sigmoid_f<DT>(f.gate[(int64_t)group * f.ldgate + col]);
+        sum *= sg * (1.f - sg);
+      }
+      f.to[4][(int64_t)group * f.C + col] = sum;
+      return;
+    }
+    group = b / cols;
+    b %= cols;
+  }
+  col = b * 32 + (threadIdx.x & 31);
+  const int slice = threadIdx.x >> 5;
   float sum = 0.f;
-  if (f.to[i] && col < f.C) {
+  if (col < f.C) {
     const float* from = f.from[i] + (int64_t)group * f.parts * f.C + col;
-#pragma unroll 8
+#pragma unroll 16
     for (int r = slice; r < rows; r += 32) sum += from[(int64_t)r * f.C];
   }
   join[slice][threadIdx.x & 31] = sum;
   __syncthreads();
-  if (slice == 0 && f.to[i] && col < f.C) {
+  if (slice == 0 && col < f.C) {
     sum = 0.f;
 #pragma unroll
     for (int q = 0; q < 32; ++q) sum += join[q][threadIdx.x];
@@ -574,29 +718,35 @@ void launch_residual_norm_bwd(const ResidualNormParams& p, hipStream_t s) {
   if (!p.dz && !p.dh) throw std::invalid_argument("residual_norm_grad: neither dh nor dz");
   const BwdPlan plan = plan_bwd(p);
   const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
-  float* to[5] = {p.dpre_gamma, p.dpre_beta, p.dpost_gamma, p.dpost_beta, nullptr};
+  float* to[5] = {p.dpre_gamma, p.dpost_gamma, p.dpre_beta, p.dpost_beta, nullptr};
   if (p.gate_mode == GATE_GROUP && plan.parts > 1) to[4] = reinterpret_cast<float*>(p.dgate);
   Partials part;
   Finish f;
-  bool any = false;
+  int vectors = 0;
   for (int i = 0; i < 5; ++i) {
     part.row[i] = to[i] ? p.ws + (size_t)i * plan.blocks * p.C : nullptr;
     f.from[i] = part.row[i];
     f.to[i] = to[i];
-    any = any || to[i];
+    vectors += i < 4 && to[i];
   }
-  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((bwd_kernel<DT, LPR, WIDE, K>), dim3(plan.blocks),
-                                                             dim3(threads), 0, s, p, plan, part)));
-  if (!any) return;
+#define DTF_BWD(LAYER, GROUP)                                                                                  \
+  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((bwd_kernel<DT, LPR, WIDE, K, LAYER, GROUP>),      \
+                                                             dim3(plan.blocks), dim3(threads), 0, s, p, plan, part)))
+  if (p.layer) {
+    if (p.gate_mode == GATE_GROUP) { DTF_BWD(true, true); } else { DTF_BWD(true, false); }
+  } else {
+    if (p.gate_mode == GATE_GROUP) { DTF_BWD(false, true); } else { DTF_BWD(false, false); }
+  }
+#undef DTF_BWD
+  if (!vectors && !to[4]) return;
   f.gate = reinterpret_cast<const float*>(p.gate);
   f.ldgate = p.ldgate;
   f.C = p.C;
   f.rows = plan.blocks;
   f.parts = plan.parts;
+  f.groups = plan.groups;
   f.sigmoid = p.sigmoid;
-  const int cols = (p.C + 31) / 32;
-  if (to[0] || to[1] || to[2] || to[3])
-    DTF_DT_SWITCH(p.dt, hipLaunchKernelGGL(finish_kernel<DT>, dim3(cols, 4, 1), dim3(1024), 0, s, f, 0));
-  if (to[4])
-    DTF_DT_SWITCH(p.dt, hipLaunchKernelGGL(finish_kernel<DT>, dim3(cols, 1, plan.groups), dim3(1024), 0, s, f, 4));
+  f.vector_blocks = vectors * ((p.C + 31) / 32);
+  const int gates = to[4] ? plan.groups * (plan.parts <= FEW_PARTS ? (p.C + 1023) / 1024 : (p.C + 31) / 32) : 0;
+  DTF_DT_SWITCH(p.dt, hipLaunchKernelGGL(finish_kernel<DT>, dim3(f.vector_blocks + gates), dim3(1024), 0, s, f));
 }

@@ -44,15 +44,12 @@ def sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity: torch.T
 MAX_CHANNELS = 8192      # of the native kernels
 
 
-def _pitch(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
-  """Elements from one row of `t` to the next; rows are everything but the last dimension."""
-  if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-    raise ValueError("%s: %s %s on %s, but the rows are %s %s on %s" % (
-        name, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
-  return _row_pitch(name, t)
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_FP32 = torch.float32
 
 
 def _row_pitch(name: str, t: torch.Tensor) -> int:
+  """Elements from one row of `t` to the next; rows are everything but the last dimension."""
   channels = t.shape[-1]
   if t.is_contiguous():
     return channels
@@ -60,66 +57,76 @@ def _row_pitch(name: str, t: torch.Tensor) -> int:
     raise ValueError("%s: the channels of a row have to lie next to each other" % name)
   if t.dim() == 1:
     return channels
-  pitch = t.stride(-2)
-  for d in range(t.dim() - 2):      # the rows in front have to continue at the same pitch
+  last = t.dim() - 2
+  while last > 0 and t.shape[last] == 1:      # a dimension of one row has no distance of its own
+    last -= 1
+  pitch = t.stride(last)
+  for d in range(last):
     if t.shape[d] > 1 and t.stride(d) != pitch * t.shape[d + 1:-1].numel():
       raise ValueError("%s: its rows lie at different distances" % name)
   return pitch
 
 
-class _Seam:
-  """Checked arguments of `residual_norm` and `residual_norm_grad`."""
+def _pitch(name: str, t: torch.Tensor, shape, dtype, device: int) -> int:
+  if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
+    raise ValueError("%s: %s %s on %s, but the rows are %s %s on device %d" % (
+        name, tuple(t.shape), t.dtype, t.device, tuple(shape), dtype, device))
+  return _row_pitch(name, t)
 
-  __slots__ = ("rows", "channels", "group_rows", "sigmoid", "layer", "gate_pitch")
 
-  def __init__(self, like, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps):
-    if like.dim() < 1 or like.shape[-1] < 1:
-      raise ValueError("rows of at least one channel, got %s" % (tuple(like.shape),))
-    if like.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-      raise ValueError("element type %s (bfloat16, float16 and float32 are built)" % like.dtype)
-    self.channels = c = like.shape[-1]
-    self.rows = like.numel() // c
-    if norm not in ("rms", "layer"):
+def _seam(like, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps):
+  """Checks what `residual_norm` and `residual_norm_grad` have in common; (rows, channels, rows that share a gate row
+  or 0, gate pitch, sigmoid, layer).  (Written for its own speed: it runs before every launch.)"""
+  shape, dtype, device = like.shape, like.dtype, like.get_device()
+  if not shape or shape[-1] < 1:
+    raise ValueError("rows of at least one channel, got %s" % (tuple(shape),))
+  if dtype not in _TYPES:
+    raise ValueError("element type %s (bfloat16, float16 and float32 are built)" % dtype)
+  c = shape[-1]
+  rows = like.numel() // c
+  layer = norm == "layer"
+  if not layer:
+    if norm != "rms":
       raise ValueError("norm is 'rms' or 'layer', not %r" % (norm,))
-    self.layer = norm == "layer"
-    if not eps > 0:
-      raise ValueError("eps has to be positive")
-    if gate_act not in ("none", "sigmoid"):
-      raise ValueError("gate_act is 'none' or 'sigmoid', not %r" % (gate_act,))
-    self.sigmoid = gate_act == "sigmoid"
-    if y is None and (post_gamma is not None or gate is not None):
-      raise ValueError("post_gamma and gate belong to y")
-    if (post_beta is not None and post_gamma is None) or (pre_beta is not None and pre_gamma is None):
-      raise ValueError("a beta goes with its gamma")
-    if not self.layer and (post_beta is not None or pre_beta is not None):
+    if post_beta is not None or pre_beta is not None:
       raise ValueError("norm='rms' has no beta")
-    for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma),
-                    ("pre_beta", pre_beta)):
-      if t is not None and (t.shape != (c,) or t.dtype != torch.float32 or t.device != like.device
-                            or not t.is_contiguous()):
-        raise ValueError("%s: %d contiguous float32 values on %s" % (name, c, like.device))
-    self.group_rows, self.gate_pitch = 0, c
-    if gate is not None:
-      if gate.dtype == like.dtype and gate.shape == like.shape:
-        self.gate_pitch = _pitch("gate", gate, like)
-      elif gate.dtype == torch.float32 and gate.device == like.device and gate.dim() in (1, 2) and gate.shape[-1] == c:
-        groups = gate.numel() // c
-        if groups < 1 or self.rows % groups:
-          raise ValueError("gate: %d rows of it do not divide %d rows" % (groups, self.rows))
-        self.group_rows = self.rows // groups
-        self.gate_pitch = _row_pitch("gate", gate)
-      else:
-        raise ValueError("gate: one value per element in the rows' type, or float32 [groups, %d] with groups that "
-                         "divide the rows; got %s %s on %s" % (c, tuple(gate.shape), gate.dtype, gate.device))
+  if not eps > 0:
+    raise ValueError("eps has to be positive")
+  sigmoid = gate_act == "sigmoid"
+  if not sigmoid and gate_act != "none":
+    raise ValueError("gate_act is 'none' or 'sigmoid', not %r" % (gate_act,))
+  if y is None and (post_gamma is not None or gate is not None):
+    raise ValueError("post_gamma and gate belong to y")
+  if (post_beta is not None and post_gamma is None) or (pre_beta is not None and pre_gamma is None):
+    raise ValueError("a beta goes with its gamma")
+  for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma),
+                  ("pre_beta", pre_beta)):
+    if t is not None and (t.dim() != 1 or t.numel() != c or t.dtype is not _FP32 or t.get_device() != device
+                          or not t.is_contiguous()):
+      raise ValueError("%s: %d contiguous float32 values on the rows' device" % (name, c))
+  group_rows, gate_pitch = 0, c
+  if gate is not None:
+    if gate.dtype is dtype and gate.shape == shape:
+      gate_pitch = _pitch("gate", gate, shape, dtype, device)
+    elif gate.dtype is _FP32 and gate.get_device() == device and gate.dim() in (1, 2) and gate.shape[-1] == c:
+      groups = gate.numel() // c
+      if groups < 1 or rows % groups:
+        raise ValueError("gate: %d rows of it do not divide %d rows" % (groups, rows))
+      group_rows = rows // groups
+      gate_pitch = _row_pitch("gate", gate)
+    else:
+      raise ValueError("gate: one value per element in the rows' type, or float32 [groups, %d] with groups that "
+                       "divide the rows; got %s %s on %s" % (c, tuple(gate.shape), gate.dtype, gate.device))
+  return rows, c, group_rows, gate_pitch, sigmoid, layer
 
 
-def _no_graph(**tensors):
+def _no_graph(*tensors):
   """These entry points compute values; a gradient that autograd would have to record is refused, not lost."""
   if torch.is_grad_enabled():
-    for name, t in tensors.items():
+    for t in tensors:
       if t is not None and t.requires_grad:
-        raise ValueError("%s requires a gradient: it is computed by residual_norm_grad, call under torch.no_grad()"
-                         % name)
+        raise ValueError("an argument requires a gradient: it is computed by residual_norm_grad, call under "
+                         "torch.no_grad()")
 
 
 def _normalised(v: torch.Tensor, layer: bool, eps: float):
@@ -134,11 +141,11 @@ def _normalised_grad(d, hat, r, layer):
   return r * (d - d_mean - hat * (d * hat).mean(-1, keepdim=True))
 
 
-def _gate_factor(s: _Seam, gate):
+def _gate_factor(gate, rows, channels, group_rows, sigmoid):
   """The gate's factor per row and its derivative, in float32."""
-  g = gate.float().reshape(-1, s.channels)
-  g = g.repeat_interleave(s.group_rows, 0) if s.group_rows else g[:s.rows]
-  if not s.sigmoid:
+  g = gate.float().reshape(-1, channels)
+  g = g.repeat_interleave(group_rows, 0) if group_rows else g[:rows]
+  if not sigmoid:
     return g, 1.0
   a = torch.sigmoid(g)
   return a, a * (1 - a)
@@ -162,30 +169,30 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_gam
   are summed in float32: a row whose values pass 1e18 overflows there.
   No graph is recorded; `residual_norm_grad` is the gradient.
   """
-  s = _Seam(x, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps)
-  _no_graph(x=x, y=y, post_gamma=post_gamma, post_beta=post_beta, gate=gate, pre_gamma=pre_gamma, pre_beta=pre_beta)
-  pitch = dict(x=_row_pitch("x", x), gate=s.gate_pitch)
-  if y is not None:
-    pitch["y"] = _pitch("y", y, x)
-  if x.device.type == "cuda":
-    if s.channels > MAX_CHANNELS:
-      raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, s.channels))
+  rows, c, group_rows, ldgate, sigmoid, layer = _seam(x, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta,
+                                                      norm, eps)
+  _no_graph(x, y, post_gamma, post_beta, gate, pre_gamma, pre_beta)
+  ldx = _row_pitch("x", x)
+  ldy = c if y is None else _pitch("y", y, x.shape, x.dtype, x.get_device())
+  if x.is_cuda:
+    if c > MAX_CHANNELS:
+      raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, c))
     from . import native  # pylint: disable=import-outside-toplevel
-    return native.residual_norm(x, y, s.rows, s.channels, pitch, gate, s.group_rows, s.sigmoid, s.layer,
-                                float(residual_scale), float(eps), post_gamma, post_beta, pre_gamma, pre_beta)
-  h, z = x.float().reshape(-1, s.channels), None
+    return native.residual_norm(x, ldx, y, ldy, rows, c, gate, ldgate, group_rows, sigmoid, layer, residual_scale, eps,
+                                post_gamma, post_beta, pre_gamma, pre_beta)
+  h, z = x.float().reshape(-1, c), None
   out = x
   if y is not None:
-    n = y.float().reshape(-1, s.channels)
+    n = y.float().reshape(-1, c)
     if post_gamma is not None:
-      n = _normalised(n, s.layer, eps)[0] * post_gamma
+      n = _normalised(n, layer, eps)[0] * post_gamma
       n = n if post_beta is None else n + post_beta
     if gate is not None:
-      n = n * _gate_factor(s, gate)[0]
+      n = n * _gate_factor(gate, rows, c, group_rows, sigmoid)[0]
     h = h + residual_scale * n
     out = h.to(x.dtype).view(x.shape)
   if pre_gamma is not None:
-    z = _normalised(h, s.layer, eps)[0] * pre_gamma
+    z = _normalised(h, layer, eps)[0] * pre_gamma
     z = (z if pre_beta is None else z + pre_beta).to(x.dtype).view(x.shape)
   return out, z
 
@@ -202,55 +209,55 @@ def residual_norm_grad(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], h
   given.  The norms' statistics are taken from h and y again, so nothing has to be kept from the forward call.
   Sums over rows are float32 in a fixed order: the same call gives the same bits.
   """
-  s = _Seam(h, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps)
-  _no_graph(dh=dh, dz=dz, h=h, y=y, post_gamma=post_gamma, post_beta=post_beta, gate=gate, pre_gamma=pre_gamma,
-            pre_beta=pre_beta)
+  rows, c, group_rows, ldgate, sigmoid, layer = _seam(h, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta,
+                                                      norm, eps)
+  _no_graph(dh, dz, h, y, post_gamma, post_beta, gate, pre_gamma, pre_beta)
   if (dz is None) != (pre_gamma is None):
     raise ValueError("dz goes with pre_gamma")
   if dz is None and dh is None:
     raise ValueError("neither dh nor dz")
-  pitch = dict(h=_row_pitch("h", h), gate=s.gate_pitch)
-  for name, t in (("dh", dh), ("dz", dz), ("y", y)):
-    if t is not None:
-      pitch[name] = _pitch(name, t, h)
-  if h.device.type == "cuda":
-    if s.channels > MAX_CHANNELS:
-      raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, s.channels))
+  shape, dtype, device = h.shape, h.dtype, h.get_device()
+  ldh = _row_pitch("h", h)
+  lddh = c if dh is None else _pitch("dh", dh, shape, dtype, device)
+  lddz = c if dz is None else _pitch("dz", dz, shape, dtype, device)
+  ldy = c if y is None else _pitch("y", y, shape, dtype, device)
+  if h.is_cuda:
+    if c > MAX_CHANNELS:
+      raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, c))
     from . import native  # pylint: disable=import-outside-toplevel
-    return native.residual_norm_grad(dh, dz, h, y, s.rows, s.channels, pitch, gate, s.group_rows, s.sigmoid, s.layer,
-                                     float(residual_scale), float(eps), post_gamma, post_beta, pre_gamma, pre_beta)
-  c = s.channels
+    return native.residual_norm_grad(dh, lddh, dz, lddz, h, ldh, y, ldy, rows, c, gate, ldgate, group_rows, sigmoid,
+                                     layer, residual_scale, eps, post_gamma, post_beta, pre_gamma, pre_beta)
   out: Dict[str, Optional[torch.Tensor]] = dict.fromkeys(
       ("dx", "dy", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"))
-  up = dh.float().reshape(-1, c) if dh is not None else torch.zeros(s.rows, c)
+  up = dh.float().reshape(-1, c) if dh is not None else torch.zeros(rows, c)
   if dz is not None:
     d = dz.float().reshape(-1, c)
-    hat, r = _normalised(h.float().reshape(-1, c), s.layer, eps)
+    hat, r = _normalised(h.float().reshape(-1, c), layer, eps)
     out["dpre_gamma"] = (d * hat).sum(0)
     if pre_beta is not None:
       out["dpre_beta"] = d.sum(0)
-    up = up + _normalised_grad(d * pre_gamma, hat, r, s.layer)
+    up = up + _normalised_grad(d * pre_gamma, hat, r, layer)
   out["dx"] = up.to(h.dtype).view(h.shape)
   if y is None:
     return out
   up = residual_scale * up
   n = y.float().reshape(-1, c)
   if post_gamma is not None:
-    hat, r = _normalised(n, s.layer, eps)
+    hat, r = _normalised(n, layer, eps)
     n = hat * post_gamma
     n = n if post_beta is None else n + post_beta
   if gate is not None:
-    a, slope = _gate_factor(s, gate)
+    a, slope = _gate_factor(gate, rows, c, group_rows, sigmoid)
     dg = up * n * slope
-    if s.group_rows or not s.rows:
-      dg = dg.view(gate.numel() // c, -1, c).sum(1) if s.rows else torch.zeros(gate.shape)
+    if group_rows or not rows:
+      dg = dg.view(gate.numel() // c, -1, c).sum(1) if rows else torch.zeros(gate.shape)
     out["dgate"] = dg.to(gate.dtype).view(gate.shape)
     up = up * a
   if post_gamma is not None:
     out["dpost_gamma"] = (up * hat).sum(0)
     if post_beta is not None:
       out["dpost_beta"] = up.sum(0)
-    up = _normalised_grad(up * post_gamma, hat, r, s.layer)
+    up = _normalised_grad(up * post_gamma, hat, r, layer)
   out["dy"] = up.to(h.dtype).view(h.shape)
   return out
 
@@ -302,11 +309,12 @@ class TensorTable:
     outs = [_span(o) for o in self.out]
     apart = [_span(t) for t, o in zip(self.tensors, self.out) if t.data_ptr() != o.data_ptr()]
     self._clash = _overlaps(outs) or (bool(apart) and _overlaps_two(outs, apart))
-    self._list = None
+    self.list, self.workspace = None, 0        # native: the launches' tables, doubles they need
     if self.device.type == "cuda":
       from . import native  # pylint: disable=import-outside-toplevel
-      self._list = native.ext().ClipList(self._at, self._to, [t.numel() for t in self.tensors],
+      self.list = native.ext().ClipList(self._at, self._to, [t.numel() for t in self.tensors],
                                          [native.dtype_code(t.dtype) for t in self.tensors])
+      self.workspace = max(self.list.workspace_doubles, 1)
 
   def _current(self) -> "TensorTable":
     if self._at != list(map(torch.Tensor.data_ptr, self.tensors)) or (

@@ -6,7 +6,6 @@ device path never falls back to library kernels silently.
 """
 from __future__ import annotations
 
-import contextlib
 import struct
 from typing import Dict, List, Optional, Sequence
 
@@ -77,125 +76,109 @@ def dtype_code(dtype: torch.dtype) -> int:
     raise ValueError("element type %s (bfloat16, float16 and float32 are built)" % dtype) from None
 
 
-@contextlib.contextmanager
-def _on_device(device: torch.device):
-  """The device's current stream; kernels of another device than the current one are launched from there."""
-  if device.index is None or device.index == torch.cuda.current_device():
-    yield stream_handle()
-  else:
-    with torch.cuda.device(device):
-      yield stream_handle()
+def _elsewhere(index: int) -> bool:
+  """Whether device `index` is not the current one: its kernels are then launched from `torch.cuda.device(index)`."""
+  return index != torch.cuda.current_device()
+
+
+# raw hipStream_t of a device's current stream, without a Stream object (0.1 instead of 2.8 us)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity: torch.Tensor, l2x2: torch.Tensor,
                             lr: float, momentum: float, clip_norm: float, grad_scale: float = 1.0,
                             skip: Optional[torch.Tensor] = None) -> torch.Tensor:
   """Two launches: the norm's partial sums, the update (arguments checked by `fused`)."""
+  index = params.get_device()
+  if _elsewhere(index):
+    with torch.cuda.device(index):
+      return clipped_sgd_momentum_l2(params, grads, velocity, l2x2, lr, momentum, clip_norm, grad_scale, skip)
   n = params.numel()
-  dev = params.device
-  with _on_device(dev) as stream:
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(ext().clipped_sgd_blocks(n), dtype=torch.float64, device=dev)
-    run_op("clipped_sgd", dict(p=params.data_ptr(), g=grads.data_ptr(), v=velocity.data_ptr(),
-                               l2x2=l2x2.data_ptr(), n=n, lr=float(lr), momentum=float(momentum),
-                               clip=float(clip_norm), grad_scale=float(grad_scale),
-                               skip=skip.data_ptr() if skip is not None else None,
-                               ws=ws.data_ptr(), norm=norm.data_ptr()), stream)
+  norm = params.new_empty(())
+  ws = params.new_empty(ext().clipped_sgd_blocks(n), dtype=torch.float64)
+  ext().clipped_sgd(params.data_ptr(), grads.data_ptr(), velocity.data_ptr(), l2x2.data_ptr(), n, lr, momentum,
+                    grad_scale, clip_norm, skip.data_ptr() if skip is not None else 0, ws.data_ptr(),
+                    norm.data_ptr(), _current_stream(index))
   return norm
 
 
 def clip_list_norm(table) -> torch.Tensor:
   """Global norm of a `fused.TensorTable`.  The workspace is the call's own: tables are shared between streams."""
-  lst, dev = table._list, table.device
-  with _on_device(dev) as stream:
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(max(lst.workspace_doubles, 1), dtype=torch.float64, device=dev)
-    lst.global_norm(ws.data_ptr(), norm.data_ptr(), stream)
+  index = table.device.index
+  if _elsewhere(index):
+    with torch.cuda.device(index):
+      return clip_list_norm(table)
+  norm = torch.empty((), dtype=torch.float32, device=table.device)
+  ws = torch.empty(table.workspace, dtype=torch.float64, device=table.device)
+  table.list.global_norm(ws.data_ptr(), norm.data_ptr(), _current_stream(index))
   return norm
 
 
 def clip_list_scale(table, clip_norm: float, use_norm: Optional[torch.Tensor]) -> torch.Tensor:
   """Clips a `fused.TensorTable` into its outputs; the norm."""
-  lst, dev = table._list, table.device
-  with _on_device(dev) as stream:
-    if use_norm is not None:
-      lst.clip(0, use_norm.data_ptr(), clip_norm, 0, stream)
-      return use_norm
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(max(lst.workspace_doubles, 1), dtype=torch.float64, device=dev)
-    lst.clip(ws.data_ptr(), 0, clip_norm, norm.data_ptr(), stream)
+  index = table.device.index
+  if _elsewhere(index):
+    with torch.cuda.device(index):
+      return clip_list_scale(table, clip_norm, use_norm)
+  if use_norm is not None:
+    table.list.clip(0, use_norm.data_ptr(), clip_norm, 0, _current_stream(index))
+    return use_norm
+  norm = torch.empty((), dtype=torch.float32, device=table.device)
+  ws = torch.empty(table.workspace, dtype=torch.float64, device=table.device)
+  table.list.clip(ws.data_ptr(), 0, clip_norm, norm.data_ptr(), _current_stream(index))
   return norm
 
 
-def _vectors(args: Dict, post_gamma, post_beta, pre_gamma, pre_beta):
-  if post_gamma is not None:
-    args["post_gamma"] = post_gamma.data_ptr()
-    if post_beta is not None:
-      args["post_beta"] = post_beta.data_ptr()
-  if pre_gamma is not None:
-    args["pre_gamma"] = pre_gamma.data_ptr()
-    if pre_beta is not None:
-      args["pre_beta"] = pre_beta.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+  return 0 if t is None else t.data_ptr()
 
 
-def residual_norm(x, y, rows: int, channels: int, pitch: Dict, gate, group_rows: int, sigmoid: bool, layer: bool,
-                  scale: float, eps: float, post_gamma, post_beta, pre_gamma, pre_beta):
-  """One launch (arguments checked by `fused`); `pitch`: elements from one row to the next."""
-  dev = x.device
-  with _on_device(dev) as stream:
-    args = dict(dt=_DT[x.dtype], P=rows, C=channels, layer=int(layer), sigmoid=int(sigmoid), scale=scale, eps=eps,
-                x=x.data_ptr(), ldx=pitch["x"])
-    h, z = x, None
-    if y is not None:
-      h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-      args.update(y=y.data_ptr(), ldy=pitch["y"], h=h.data_ptr())
-      if gate is not None:
-        args.update(gate=gate.data_ptr(), ldgate=pitch["gate"], group_rows=group_rows)
-    if pre_gamma is not None:
-      z = torch.empty(x.shape, dtype=x.dtype, device=dev)
-      args["z"] = z.data_ptr()
-    _vectors(args, post_gamma, post_beta, pre_gamma, pre_beta)
-    if rows and (h is not x or z is not None):
-      run_op("residual_norm_fwd", args, stream)
+def residual_norm(x, ldx, y, ldy, rows, channels, gate, ldgate, group_rows, sigmoid, layer, scale, eps, post_gamma,
+                  post_beta, pre_gamma, pre_beta):
+  """One launch (arguments checked by `fused`); ld*: elements from one row to the next."""
+  index = x.get_device()
+  if _elsewhere(index):
+    with torch.cuda.device(index):
+      return residual_norm(x, ldx, y, ldy, rows, channels, gate, ldgate, group_rows, sigmoid, layer, scale, eps,
+                           post_gamma, post_beta, pre_gamma, pre_beta)
+  h = x if y is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+  z = None if pre_gamma is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+  if rows and (h is not x or z is not None):
+    ext().residual_norm_fwd(_DT[x.dtype], rows, channels, layer, sigmoid, scale, eps, x.data_ptr(), ldx, _ptr(y), ldy,
+                            _ptr(gate), ldgate, group_rows, _ptr(post_gamma), _ptr(post_beta), _ptr(pre_gamma),
+                            _ptr(pre_beta), h.data_ptr(), _ptr(z), _current_stream(index))
   return h, z
 
 
-def residual_norm_grad(dh, dz, h, y, rows: int, channels: int, pitch: Dict, gate, group_rows: int, sigmoid: bool,
-                       layer: bool, scale: float, eps: float, post_gamma, post_beta, pre_gamma, pre_beta) -> Dict:
-  """The sweep over the rows and, where sums over rows are asked for, one or two launches that finish them."""
-  dev = h.device
-  with _on_device(dev) as stream:
-    def rows_like():
-      return torch.empty(h.shape, dtype=h.dtype, device=dev)
-
-    # the four vectors' gradients sit in one buffer
-    names = [n for n, t in (("pre_gamma", pre_gamma), ("pre_beta", pre_beta), ("post_gamma", post_gamma),
-                            ("post_beta", post_beta)) if t is not None]
-    make = torch.empty if rows else torch.zeros
-    vectors = make((max(len(names), 1), channels), dtype=torch.float32, device=dev)
-    out = dict(dx=rows_like(), dy=None, dgate=None, dpost_gamma=None, dpost_beta=None, dpre_gamma=None,
-               dpre_beta=None)
-    for i, n in enumerate(names):
-      out["d" + n] = vectors[i]
-    if y is not None:
-      out["dy"] = rows_like()
-    if gate is not None:
-      out["dgate"] = make(gate.shape, dtype=gate.dtype, device=dev)
-    if rows:
-      ws = torch.empty(ext().residual_norm_workspace_floats(rows, channels, group_rows), dtype=torch.float32, device=dev)
-      args = dict(dt=_DT[h.dtype], P=rows, C=channels, layer=int(layer), sigmoid=int(sigmoid), scale=scale, eps=eps,
-                  ws=ws.data_ptr())
-      for n, t in (("dh", dh), ("dz", dz), ("h", h), ("y", y), ("gate", gate)):
-        if t is not None:
-          args[n] = t.data_ptr()
-          args["ld" + n] = pitch[n]
-      if gate is not None:
-        args["group_rows"] = group_rows
-      _vectors(args, post_gamma, post_beta, pre_gamma, pre_beta)
-      for n, t in out.items():
-        if t is not None:
-          args[n] = t.data_ptr()
-      run_op("residual_norm_bwd", args, stream)
+def residual_norm_grad(dh, lddh, dz, lddz, h, ldh, y, ldy, rows, channels, gate, ldgate, group_rows, sigmoid, layer,
+                       scale, eps, post_gamma, post_beta, pre_gamma, pre_beta) -> Dict:
+  """The sweep over the rows and, where sums over rows are asked for, one launch that finishes them."""
+  index = h.get_device()
+  if _elsewhere(index):
+    with torch.cuda.device(index):
+      return residual_norm_grad(dh, lddh, dz, lddz, h, ldh, y, ldy, rows, channels, gate, ldgate, group_rows, sigmoid,
+                                layer, scale, eps, post_gamma, post_beta, pre_gamma, pre_beta)
+  # the gradients of the four vectors sit in one buffer
+  names = [n for n, t in (("dpre_gamma", pre_gamma), ("dpre_beta", pre_beta), ("dpost_gamma", post_gamma),
+                          ("dpost_beta", post_beta)) if t is not None]
+  out = dict.fromkeys(("dx", "dy", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"))
+  vectors = None
+  if names:
+    vectors = (h.new_empty if rows else h.new_zeros)((len(names), channels), dtype=torch.float32)
+    out.update(zip(names, vectors.unbind(0)))
+  dx = out["dx"] = torch.empty_like(h, memory_format=torch.contiguous_format)
+  dy = out["dy"] = None if y is None else torch.empty_like(h, memory_format=torch.contiguous_format)
+  dgate = None
+  if gate is not None:
+    dgate = (torch.empty_like if rows else torch.zeros_like)(gate, memory_format=torch.contiguous_format)
+    out["dgate"] = dgate
+  if rows:
+    e = ext()
+    ws = h.new_empty(e.residual_norm_workspace_floats(rows, channels, group_rows), dtype=torch.float32)
+    e.residual_norm_bwd(_DT[h.dtype], rows, channels, layer, sigmoid, scale, eps, h.data_ptr(), ldh, _ptr(y), ldy,
+                        _ptr(gate), ldgate, group_rows, _ptr(post_gamma), _ptr(post_beta), _ptr(pre_gamma),
+                        _ptr(pre_beta), _ptr(dh), lddh, _ptr(dz), lddz, dx.data_ptr(), _ptr(dy), _ptr(dgate),
+                        _ptr(vectors), ws.data_ptr(), _current_stream(index))
   return out
 
 
