@@ -842,9 +842,9 @@ PYBIND11_MODULE(_dtf_native, m) {
     launch_residual_norm_bwd(p, reinterpret_cast<hipStream_t>(stream));
     check_launch();
   });
-  m.def("residual_norm_workspace_floats", [](int P, int C, int group_rows) {
+  m.def("residual_norm_workspace_floats", [](int P, int C, int group_rows, int dt, int layer) {
     ResidualNormParams p;
-    p.P = P; p.C = C; p.group_rows = group_rows;
+    p.P = P; p.C = C; p.group_rows = group_rows; p.dt = dt; p.layer = layer;
     p.gate_mode = group_rows > 0 ? GATE_GROUP : GATE_NONE;
     return residual_norm_workspace_floats(p);
   }, "Floats that residual_norm_bwd keeps its partial sums in; group_rows: rows that share a gate row, or 0");

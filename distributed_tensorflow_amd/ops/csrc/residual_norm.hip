@@ -21,19 +21,31 @@
 namespace {
 
 // 16 bytes at the alignment of their elements: the memory system takes any address, one load all the same
-struct __attribute__((packed, aligned(2))) Any16 { u32x4 v; };
-struct __attribute__((packed, aligned(4))) Any16F { f32x4 v; };
+typedef u32x4 __attribute__((aligned(2))) Any16;
+typedef f32x4 __attribute__((aligned(4))) Any16F;
+
+// NT: past the caches (a sweep over more than they hold)
+template <bool NT, typename V>
+__device__ __forceinline__ V get16(const V* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool NT, typename V, typename W>
+__device__ __forceinline__ void put16(V* p, const W v) {
+  if constexpr (NT) __builtin_nontemporal_store((V)v, p);
+  else *p = v;
+}
 
 // Eight channels from `c` on of the row at `p`, as they sit in memory; what lies past channel C - 1 is zero.
-template <int DT>
+template <int DT, bool NT = false>
 __device__ __forceinline__ Raw8<DT> load_raw(const typename Elem<DT>::T* p, int c, int C) {
   Raw8<DT> r = zero_raw<DT>();
   if (c + 8 <= C) {
     if constexpr (DT == DT_F32) {
-      r.lo = reinterpret_cast<const Any16F*>(p + c)->v;
-      r.hi = reinterpret_cast<const Any16F*>(p + c + 4)->v;
+      r.lo = get16<NT>(reinterpret_cast<const Any16F*>(p + c));
+      r.hi = get16<NT>(reinterpret_cast<const Any16F*>(p + c + 4));
     } else {
-      r.v = reinterpret_cast<const Any16*>(p + c)->v;
+      r.v = get16<NT>(reinterpret_cast<const Any16*>(p + c));
     }
   } else if (c < C) {
     if constexpr (DT == DT_F32) {
@@ -56,23 +68,39 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::T* p, int c, int 
   unpack8<DT>(load_raw<DT>(p, c, C), f);
 }
 
+// Rows of the arguments; `nt` is the same for a whole launch.
 template <int DT>
+__device__ __forceinline__ void load_into(const void* from, int64_t at, int c, int C, float* f, int nt) {
+  const typename Elem<DT>::T* p = reinterpret_cast<const typename Elem<DT>::T*>(from) + at;
+  if (nt) unpack8<DT>(load_raw<DT, true>(p, c, C), f);
+  else unpack8<DT>(load_raw<DT, false>(p, c, C), f);
+}
+
+template <int DT, bool NT = false>
 __device__ __forceinline__ void store8(typename Elem<DT>::T* p, int c, int C, const float* f) {
   if (c + 8 <= C) {
     if constexpr (DT == DT_F32) {
-      reinterpret_cast<Any16F*>(p + c)->v = f32x4{f[0], f[1], f[2], f[3]};
-      reinterpret_cast<Any16F*>(p + c + 4)->v = f32x4{f[4], f[5], f[6], f[7]};
+      put16<NT>(reinterpret_cast<Any16F*>(p + c), f32x4{f[0], f[1], f[2], f[3]});
+      put16<NT>(reinterpret_cast<Any16F*>(p + c + 4), f32x4{f[4], f[5], f[6], f[7]});
     } else {
       u32x4 v;
       v.x = pack2<DT>(f[0], f[1]); v.y = pack2<DT>(f[2], f[3]);
       v.z = pack2<DT>(f[4], f[5]); v.w = pack2<DT>(f[6], f[7]);
-      reinterpret_cast<Any16*>(p + c)->v = v;
+      put16<NT>(reinterpret_cast<Any16*>(p + c), v);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (c + j < C) p[c + j] = from_f<DT>(f[j]);
   }
+}
+
+// Rows of the results; `nt` is the same for a whole launch.
+template <int DT>
+__device__ __forceinline__ void store_row(void* to, int64_t at, int c, int C, const float* f, int nt) {
+  typename Elem<DT>::T* p = reinterpret_cast<typename Elem<DT>::T*>(to) + at;
+  if (nt) store8<DT, true>(p, c, C, f);
+  else store8<DT, false>(p, c, C, f);
 }
 
 // fp32 rows take the library's exponential and a true division, 16-bit rows the hardware's (their error, a few
@@ -161,7 +189,7 @@ __device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, f
 }
 
 template <int DT, int LPR, bool WIDE, int K>
-__global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNormParams p) {
+__global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNormParams p, const int nt) {
   typedef typename Elem<DT>::T T;
   __shared__ float red[2][4][8];
   int turn = 0;
@@ -183,14 +211,14 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNor
     const int64_t r = live ? row : 0;
     float h[K][8], v[K][8];
 #pragma unroll
-    for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], Cr, h[k]);
+    for (int k = 0; k < K; ++k) load_into<DT>(p.x, r * p.ldx, c[k], Cr, h[k], nt);
     if (p.y) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], Cr, v[k]);
+      for (int k = 0; k < K; ++k) load_into<DT>(p.y, r * p.ldy, c[k], Cr, v[k], nt);
       float g[K][8];
       if (p.gate_mode == GATE_ELEMENT) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) load8<DT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], Cr, g[k]);
+        for (int k = 0; k < K; ++k) load_into<DT>(p.gate, r * p.ldgate, c[k], Cr, g[k], nt);
       } else if (p.gate_mode == GATE_GROUP) {
         const float* row_g = reinterpret_cast<const float*>(p.gate) + (r / p.group_rows) * p.ldgate;
 #pragma unroll
@@ -222,7 +250,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNor
       for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[k][j] += p.scale * (g[k][j] * v[k][j]);
-        store8<DT>(reinterpret_cast<T*>(p.h) + r * C, c[k], Cr, h[k]);
+        store_row<DT>(p.h, r * C, c[k], Cr, h[k], nt);
       }
     }
     if (p.pre_gamma) {
@@ -234,7 +262,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNor
         if (p.pre_beta) load8<DT_F32>(p.pre_beta, c[k], C, b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[k][j] = h[k][j] * rs * w[j] + b[j];
-        store8<DT>(reinterpret_cast<T*>(p.z) + r * C, c[k], Cr, h[k]);
+        store_row<DT>(p.z, r * C, c[k], Cr, h[k], nt);
       }
     }
   }
@@ -260,12 +288,28 @@ struct BwdPlan {
   int group_rows;
   int part_rows;     // rows of a group per part
   int own_groups;    // each row slot takes whole groups
+  int nt;            // more bytes than the memory-side cache holds: loads and stores past the caches
 };
+
+// Waves per SIMD that the backward kernel is built for: its registers (sums over rows, weights, a row in work and the
+// next one's loads) leave room for two, three for RMS norms of 16-bit rows.  The grid is what is resident at once:
+// one round of blocks, no half-empty second one.
+constexpr int bwd_waves(int dt, bool layer, int chunks) { return !layer && dt != DT_F32 && chunks == 1 ? 3 : 2; }
 
 int narrow_lanes(int C) {       // lanes a row of up to 512 channels
   int l = 2;
   while (l * 8 < C) l *= 2;
   return l;
+}
+
+int wide_threads(int C) {
+  const int per_wave = C <= 4096 ? 512 : 1024;
+  return 64 * ((C + per_wave - 1) / per_wave);
+}
+
+// Whether `tensors` tensors of the rows are more than the 256 MB that the memory-side cache holds.
+int big(const ResidualNormParams& p, int tensors) {
+  return (int64_t)p.P * p.C * (p.dt == DT_F32 ? 4 : 2) * tensors > (256ll << 20);
 }
 
 int fwd_blocks(int P, int slots) {
@@ -279,7 +323,9 @@ BwdPlan plan_bwd(const ResidualNormParams& p) {
   b.group_rows = grouped ? p.group_rows : p.P;
   b.groups = p.P / b.group_rows;
   const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
-  const int want = 1024;
+  const int waves = (p.C <= 512 ? 256 : wide_threads(p.C)) / 64;
+  const int want = 256 * max(1, 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2) / waves);
+  b.nt = big(p, 6);
   b.own_groups = grouped && slots > 1 && b.group_rows < 4 * slots;
   if (b.own_groups) {
     const int sets = (b.groups + slots - 1) / slots;
@@ -312,24 +358,25 @@ struct RowIn {
   Raw8<DT> dh[K], dz[K], h[K], y[K], gate[K];
 };
 
-template <int DT, int K>
+template <int DT, int K, bool NT>
 __device__ __forceinline__ void load_row(RowIn<DT, K>& in, const ResidualNormParams& p, int64_t r, const int* c, int C) {
   typedef typename Elem<DT>::T T;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     in.dh[k] = zero_raw<DT>();
-    if (p.dh) in.dh[k] = load_raw<DT>(reinterpret_cast<const T*>(p.dh) + r * p.lddh, c[k], C);
+    if (p.dh) in.dh[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.dh) + r * p.lddh, c[k], C);
     if (p.dz) {
-      in.dz[k] = load_raw<DT>(reinterpret_cast<const T*>(p.dz) + r * p.lddz, c[k], C);
-      in.h[k] = load_raw<DT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], C);
+      in.dz[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.dz) + r * p.lddz, c[k], C);
+      in.h[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], C);
     }
-    if (p.y) in.y[k] = load_raw<DT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
-    if (p.gate_mode == GATE_ELEMENT) in.gate[k] = load_raw<DT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
+    if (p.y) in.y[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
+    if (p.gate_mode == GATE_ELEMENT)
+      in.gate[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
   }
 }
 
 template <int DT, int LPR, bool WIDE, int K, bool LAYER, bool GROUP>
-__global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
+__global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
                                                                const Partials part) {
   typedef typename Elem<DT>::T T;
   // sums over rows: of the two gammas, with LAYER of the two betas, with GROUP of the gate
@@ -337,6 +384,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
   __shared__ float red[2][4][8];
   __shared__ float join[WIDE ? 1 : 256 * 8];
   int turn = 0;
+  const int nt = plan.nt;
   const int lanes = WIDE ? (int)blockDim.x : LPR;
   const int waves = WIDE ? (int)(blockDim.x >> 6) : 1;
   const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x % LPR);
@@ -398,7 +446,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
     int C_next = 0;
     if (row0 < row1) {
       C_next = row_of(row0, &r_next);
-      load_row<DT, K>(next, p, r_next, c, C_next);
+      if (nt) load_row<DT, K, true>(next, p, r_next, c, C_next);
+      else load_row<DT, K, false>(next, p, r_next, c, C_next);
     }
     for (int rr = row0; rr < row1; rr += step) {
       const RowIn<DT, K> in = next;
@@ -406,7 +455,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
       const int Cr = C_next;
       if (rr + step < row1) {          // the next row's loads are under way while this row's sums are taken
         C_next = row_of(rr + step, &r_next);
-        load_row<DT, K>(next, p, r_next, c, C_next);
+        if (nt) load_row<DT, K, true>(next, p, r_next, c, C_next);
+        else load_row<DT, K, false>(next, p, r_next, c, C_next);
       }
       float up[K][8], h[K][8], v[K][8];
 #pragma unroll
@@ -487,7 +537,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
         }
       }
 #pragma unroll
-      for (int k = 0; k < K; ++k) store8<DT>(reinterpret_cast<T*>(p.dx) + r * C, c[k], Cr, up[k]);
+      for (int k = 0; k < K; ++k) store_row<DT>(p.dx, r * C, c[k], Cr, up[k], nt);
       if (!p.y) continue;
       float t[2] = {0.f, 0.f};
 #pragma unroll
@@ -522,7 +572,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
           t[1] += up[k][j];
         }
         if constexpr (!GROUP) {
-          if (p.gate_mode == GATE_ELEMENT) store8<DT>(reinterpret_cast<T*>(p.dgate) + r * C, c[k], Cr, dg);
+          if (p.gate_mode == GATE_ELEMENT) store_row<DT>(p.dgate, r * C, c[k], Cr, dg, nt);
         }
       }
       if (p.post_gamma) {
@@ -534,7 +584,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void bwd_kernel(const ResidualNor
           for (int j = 0; j < 8; ++j) up[k][j] = rs * (up[k][j] - m_t - v[k][j] * m_dot);
       }
 #pragma unroll
-      for (int k = 0; k < K; ++k) store8<DT>(reinterpret_cast<T*>(p.dy) + r * C, c[k], Cr, up[k]);
+      for (int k = 0; k < K; ++k) store_row<DT>(p.dy, r * C, c[k], Cr, up[k], nt);
     }
     if (GROUP && plan.parts == 1) {
       // whole groups: the gate's gradient is complete here
@@ -689,10 +739,6 @@ void check(const ResidualNormParams& p) {
     else { constexpr int LPR = 64, K = 2; constexpr bool WIDE = true; __VA_ARGS__; }                \
   } while (0)
 
-int wide_threads(int C) {
-  const int per_wave = C <= 4096 ? 512 : 1024;
-  return 64 * ((C + per_wave - 1) / per_wave);
-}
 
 }  // namespace
 
@@ -707,7 +753,7 @@ void launch_residual_norm_fwd(const ResidualNormParams& p, hipStream_t s) {
   const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
   const int blocks = fwd_blocks(p.P, p.C <= 512 ? 256 / narrow_lanes(p.C) : 1);
   DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((fwd_kernel<DT, LPR, WIDE, K>), dim3(blocks), dim3(threads),
-                                                             0, s, p)));
+                                                             0, s, p, big(p, 4))));
 }
 
 void launch_residual_norm_bwd(const ResidualNormParams& p, hipStream_t s) {

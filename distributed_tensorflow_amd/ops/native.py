@@ -174,7 +174,7 @@ def residual_norm_grad(dh, lddh, dz, lddz, h, ldh, y, ldy, rows, channels, gate,
     out["dgate"] = dgate
   if rows:
     e = ext()
-    ws = h.new_empty(e.residual_norm_workspace_floats(rows, channels, group_rows), dtype=torch.float32)
+    ws = h.new_empty(e.residual_norm_workspace_floats(rows, channels, group_rows, _DT[h.dtype], layer), dtype=torch.float32)
     e.residual_norm_bwd(_DT[h.dtype], rows, channels, layer, sigmoid, scale, eps, h.data_ptr(), ldh, _ptr(y), ldy,
                         _ptr(gate), ldgate, group_rows, _ptr(post_gamma), _ptr(post_beta), _ptr(pre_gamma),
                         _ptr(pre_beta), _ptr(dh), lddh, _ptr(dz), lddz, dx.data_ptr(), _ptr(dy), _ptr(dgate),

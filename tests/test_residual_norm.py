@@ -464,7 +464,7 @@ def test_gpu_as_entries_of_a_launch_plan():
   t, kw = make("cuda", rows, c, torch.bfloat16, "rms", gate="element")
   h, z, dx, dy, dg = (torch.zeros(rows, c, dtype=torch.bfloat16, device="cuda") for _ in range(5))
   v = torch.zeros(2, c, device="cuda")
-  ws = torch.zeros(native.ext().residual_norm_workspace_floats(rows, c, 0), device="cuda")
+  ws = torch.zeros(native.ext().residual_norm_workspace_floats(rows, c, 0, 0, 0), device="cuda")
   common = dict(dt=0, P=rows, C=c, scale=0.7, eps=1e-5, y=t["y"].data_ptr(), gate=kw["gate"].data_ptr(),
                 post_gamma=kw["post_gamma"].data_ptr(), pre_gamma=kw["pre_gamma"].data_ptr())
   plan = native.Plan()
