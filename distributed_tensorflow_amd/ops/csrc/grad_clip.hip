@@ -23,7 +23,7 @@ namespace {
 
 constexpr int TPB = 256;
 constexpr int CHUNK_BYTES = TPB * 16 * 4;
-constexpr int MAX_BLOCKS = 1024;      // per launch: four blocks a CU
+constexpr int MAX_BLOCKS = 2048;      // per launch: eight blocks a CU, all its waves
 
 struct __attribute__((packed, aligned(2))) Any16 { u32x4 v; };
 
@@ -213,15 +213,27 @@ __global__ __launch_bounds__(TPB) void sgd_norm_kernel(const float* __restrict__
   unscale(skip, &grad_scale);
   const size_t n4 = n / 4, stride = (size_t)gridDim.x * TPB;
   double s[4] = {0., 0., 0., 0.};
-  for (size_t i = blockIdx.x * (size_t)TPB + threadIdx.x; i < n4; i += stride) {
-    const f32x4 w = reinterpret_cast<const f32x4*>(p)[i], gr = reinterpret_cast<const f32x4*>(g)[i];
-    const f32x4 l2 = reinterpret_cast<const f32x4*>(l2x2)[i];
+  auto take = [&](const f32x4 w, const f32x4 gr, const f32x4 l2) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double d = (double)(gr[j] * grad_scale + l2[j] * w[j]);
       s[j] = fma(d, d, s[j]);
     }
+  };
+  size_t i = blockIdx.x * (size_t)TPB + threadIdx.x;
+  for (; i + 3 * stride < n4; i += 4 * stride) {       // twelve loads under way
+    f32x4 w[4], gr[4], l2[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = reinterpret_cast<const f32x4*>(p)[i + k * stride];
+      gr[k] = reinterpret_cast<const f32x4*>(g)[i + k * stride];
+      l2[k] = reinterpret_cast<const f32x4*>(l2x2)[i + k * stride];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) take(w[k], gr[k], l2[k]);
   }
+  for (; i < n4; i += stride)
+    take(reinterpret_cast<const f32x4*>(p)[i], reinterpret_cast<const f32x4*>(g)[i], reinterpret_cast<const f32x4*>(l2x2)[i]);
   const size_t t = n4 * 4 + threadIdx.x;
   if (blockIdx.x == 0 && t < n) {
     const double d = (double)(g[t] * grad_scale + l2x2[t] * p[t]);

@@ -14,6 +14,7 @@
 // or two chunks of eight channels a lane, and join their sums through LDS.
 //
 // Loads take any alignment (rows of odd length start anywhere); the last, partial chunk of a row goes element by element.
+#include <algorithm>
 #include <stdexcept>
 
 #include "residual_norm.h"
@@ -66,14 +67,6 @@ __device__ __forceinline__ Raw8<DT> load_raw(const typename Elem<DT>::T* p, int 
 template <int DT>
 __device__ __forceinline__ void load8(const typename Elem<DT>::T* p, int c, int C, float* f) {
   unpack8<DT>(load_raw<DT>(p, c, C), f);
-}
-
-// Rows of the arguments; `nt` is the same for a whole launch.
-template <int DT>
-__device__ __forceinline__ void load_into(const void* from, int64_t at, int c, int C, float* f, int nt) {
-  const typename Elem<DT>::T* p = reinterpret_cast<const typename Elem<DT>::T*>(from) + at;
-  if (nt) unpack8<DT>(load_raw<DT, true>(p, c, C), f);
-  else unpack8<DT>(load_raw<DT, false>(p, c, C), f);
 }
 
 template <int DT, bool NT = false>
@@ -161,23 +154,37 @@ __device__ __forceinline__ void row_sums(float* v, float (*red)[4][8], int waves
   }
 }
 
-// Centres `v` (layer) and returns 1 / sqrt(mean square + eps) of the row.
-template <int LPR, bool WIDE, int K>
-__device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, float inv_c, int layer, float eps,
+// Subtracts the mean of the row from its channels (and leaves those past the end zero).
+template <int K>
+__device__ __forceinline__ void centre(float (*v)[8], const int* c, int C, float mean) {
+  if (C % 8 == 0) {       // a lane's channels are all there or none is
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float m = c[k] < C ? mean : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] -= m;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = c[k] + j < C ? v[k][j] - mean : 0.f;
+  }
+}
+
+// Centres `v` (LAYER) and returns 1 / sqrt(mean square + eps) of the row.
+template <int LPR, bool WIDE, int K, bool LAYER>
+__device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, float inv_c, float eps,
                                            float (*red)[4][8], int waves, int& turn) {
   float s[1];
-  if (layer) {
+  if constexpr (LAYER) {
     s[0] = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[0] += v[k][j];
     row_sums<LPR, WIDE, 1>(s, red, waves, turn);
-    const float mean = s[0] * inv_c;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] = c[k] + j < C ? v[k][j] - mean : 0.f;
+    centre<K>(v, c, C, s[0] * inv_c);
   }
   s[0] = 0.f;
 #pragma unroll
@@ -188,9 +195,31 @@ __device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, f
   return 1.f / sqrtf(s[0] * inv_c + eps);
 }
 
-template <int DT, int LPR, bool WIDE, int K>
-__global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNormParams p, const int nt) {
+template <int DT, int K>
+struct FwdIn {
+  Raw8<DT> x[K], y[K], gate[K];
+};
+
+template <int DT, int K, bool NT>
+__device__ __forceinline__ void load_fwd(FwdIn<DT, K>& in, const ResidualNormParams& p, int64_t r, const int* c, int C) {
   typedef typename Elem<DT>::T T;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    in.x[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], C);
+    if (p.y) in.y[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
+    if (p.gate_mode == GATE_ELEMENT)
+      in.gate[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
+  }
+}
+
+// A block takes a run of consecutive rows: while one row's sums are taken the next one's loads are under way, the
+// vectors stay in registers, and a gate row is read again only where its group ends.
+// Waves per SIMD that its registers allow; the grid is what is resident at once.
+constexpr int fwd_waves(int dt, bool layer, int chunks) { return chunks > 1 ? 2 : layer && dt == DT_F32 ? 3 : 4; }
+
+template <int DT, int LPR, bool WIDE, int K, bool LAYER>
+__global__ __launch_bounds__(WIDE ? 512 : 256, fwd_waves(DT, LAYER, K)) void fwd_kernel(const ResidualNormParams p,
+                                                                                              const int nt) {
   __shared__ float red[2][4][8];
   int turn = 0;
   const int lanes = WIDE ? (int)blockDim.x : LPR;
@@ -201,50 +230,70 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNor
   const int C = p.C;
   const float inv_c = 1.f / (float)C;
   int c[K];
+  float pw[K][8], pb[K][8], qw[K][8], qb[K][8], g[K][8];
 #pragma unroll
-  for (int k = 0; k < K; ++k) c[k] = (lane + k * lanes) * 8;
-  // every lane of a wave walks the same number of passes (the sums need all of them); rows past the end are masked
-  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.P; base += (int64_t)gridDim.x * slots) {
-    const int64_t row = base + slot;
-    const bool live = row < p.P;
-    const int Cr = live ? C : 0;       // a dead row has no channels: nothing is read or written for it
-    const int64_t r = live ? row : 0;
+  for (int k = 0; k < K; ++k) {
+    c[k] = (lane + k * lanes) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { pw[k][j] = pb[k][j] = qw[k][j] = qb[k][j] = 0.f; g[k][j] = 1.f; }
+    if (p.post_gamma) load8<DT_F32>(p.post_gamma, c[k], C, pw[k]);
+    if (LAYER && p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, pb[k]);
+    if (p.pre_gamma) load8<DT_F32>(p.pre_gamma, c[k], C, qw[k]);
+    if (LAYER && p.pre_beta) load8<DT_F32>(p.pre_beta, c[k], C, qb[k]);
+  }
+  // every lane of a wave walks the same number of passes (the sums need all of them); a row past the run's end has
+  // no channels: zeros are read and nothing is written for it
+  const int64_t row0 = (int64_t)p.P * blockIdx.x / gridDim.x, row1 = (int64_t)p.P * (blockIdx.x + 1) / gridDim.x;
+  FwdIn<DT, K> next;
+  auto ask = [&](int64_t row) {
+    const int Cr = row < row1 ? C : 0;
+    const int64_t r = row < row1 ? row : 0;
+    if (nt) load_fwd<DT, K, true>(next, p, r, c, Cr);
+    else load_fwd<DT, K, false>(next, p, r, c, Cr);
+  };
+  int group = -1;
+  if (row0 < row1) ask(row0 + slot);
+  for (int64_t base = row0; base < row1; base += slots) {
+    const FwdIn<DT, K> in = next;
+    const int64_t r = base + slot < row1 ? base + slot : 0;
+    const int Cr = base + slot < row1 ? C : 0;
+    if (base + slots < row1) ask(base + slots + slot);
     float h[K][8], v[K][8];
 #pragma unroll
-    for (int k = 0; k < K; ++k) load_into<DT>(p.x, r * p.ldx, c[k], Cr, h[k], nt);
+    for (int k = 0; k < K; ++k) unpack8<DT>(in.x[k], h[k]);
     if (p.y) {
+      if (p.gate_mode == GATE_GROUP) {
+        const int now = (int)((uint32_t)r / (uint32_t)p.group_rows);
+        if (now != group) {
+          group = now;
+          const float* row_g = reinterpret_cast<const float*>(p.gate) + (int64_t)now * p.ldgate;
 #pragma unroll
-      for (int k = 0; k < K; ++k) load_into<DT>(p.y, r * p.ldy, c[k], Cr, v[k], nt);
-      float g[K][8];
-      if (p.gate_mode == GATE_ELEMENT) {
+          for (int k = 0; k < K; ++k) {
+            load8<DT_F32>(row_g, c[k], C, g[k]);
+            if (p.sigmoid) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) load_into<DT>(p.gate, r * p.ldgate, c[k], Cr, g[k], nt);
-      } else if (p.gate_mode == GATE_GROUP) {
-        const float* row_g = reinterpret_cast<const float*>(p.gate) + (r / p.group_rows) * p.ldgate;
-#pragma unroll
-        for (int k = 0; k < K; ++k) load8<DT_F32>(row_g, c[k], Cr, g[k]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[k][j] = 1.f;
-      }
-      if (p.sigmoid) {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
-      }
-      if (p.post_gamma) {
-        const float rs = normalise<LPR, WIDE, K>(v, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
+              for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
+            }
+          }
+        }
+      } else if (p.gate_mode == GATE_ELEMENT) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          float w[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          load8<DT_F32>(p.post_gamma, c[k], C, w);
-          if (p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, b);
+          unpack8<DT>(in.gate[k], g[k]);
+          if (p.sigmoid) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * rs * w[j] + b[j];
+            for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
+          }
         }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) unpack8<DT>(in.y[k], v[k]);
+      if (p.post_gamma) {
+        const float rs = normalise<LPR, WIDE, K, LAYER>(v, c, Cr, inv_c, p.eps, red, waves, turn);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] = LAYER ? v[k][j] * rs * pw[k][j] + pb[k][j] : v[k][j] * rs * pw[k][j];
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -254,14 +303,11 @@ __global__ __launch_bounds__(WIDE ? 512 : 256) void fwd_kernel(const ResidualNor
       }
     }
     if (p.pre_gamma) {
-      const float rs = normalise<LPR, WIDE, K>(h, c, Cr, inv_c, p.layer, p.eps, red, waves, turn);
+      const float rs = normalise<LPR, WIDE, K, LAYER>(h, c, Cr, inv_c, p.eps, red, waves, turn);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        float w[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        load8<DT_F32>(p.pre_gamma, c[k], C, w);
-        if (p.pre_beta) load8<DT_F32>(p.pre_beta, c[k], C, b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[k][j] = h[k][j] * rs * w[j] + b[j];
+        for (int j = 0; j < 8; ++j) h[k][j] = LAYER ? h[k][j] * rs * qw[k][j] + qb[k][j] : h[k][j] * rs * qw[k][j];
         store_row<DT>(p.z, r * C, c[k], Cr, h[k], nt);
       }
     }
@@ -312,9 +358,12 @@ int big(const ResidualNormParams& p, int tensors) {
   return (int64_t)p.P * p.C * (p.dt == DT_F32 ? 4 : 2) * tensors > (256ll << 20);
 }
 
-int fwd_blocks(int P, int slots) {
-  const int64_t want = ((int64_t)P + slots - 1) / slots;
-  return (int)(want < 8192 ? want : 8192);
+int fwd_blocks(const ResidualNormParams& p) {
+  const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
+  const int waves = (p.C <= 512 ? 256 : wide_threads(p.C)) / 64;
+  const int most = 256 * std::max(1, 4 * fwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2) / waves);
+  const int64_t want = ((int64_t)p.P + slots - 1) / slots;
+  return (int)(want < most ? want : most);
 }
 
 BwdPlan plan_bwd(const ResidualNormParams& p) {
@@ -498,13 +547,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
           row_sums<LPR, WIDE, 3>(s, red, waves, turn);
           const float mean_h = s[0] * inv_c, mean_y = p.post_gamma ? s[1] * inv_c : 0.f;
           m_d = s[2] * inv_c;
-#pragma unroll
-          for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              h[k][j] = c[k] + j < Cr ? h[k][j] - mean_h : 0.f;
-              v[k][j] = c[k] + j < Cr ? v[k][j] - mean_y : 0.f;
-            }
+          centre<K>(h, c, Cr, mean_h);
+          centre<K>(v, c, Cr, mean_y);
           s[0] = s[1] = s[2] = 0.f;
         }
 #pragma unroll
@@ -530,7 +574,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float hat = h[k][j] * rh;
-            up[k][j] += rh * (dz[j] * qw[k][j] - m_d - hat * m_dot);
+            const float d = LAYER ? dz[j] * qw[k][j] - m_d : dz[j] * qw[k][j];
+            up[k][j] += rh * (d - hat * m_dot);
             acc[0][k][j] += dz[j] * hat;
             if constexpr (LAYER) acc[2][k][j] += dz[j];
           }
@@ -548,10 +593,10 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          // a dead row or channel has h, dz, dh, y of zero; its `up` is not (the mean of dz' under LAYER)
-          const float u = c[k] + j < Cr ? p.scale * up[k][j] : 0.f;
+          // (channels past the end: gamma is zero, so they add nothing to the row's sums; their own are not stored)
+          const float u = p.scale * up[k][j];
           const float hat = v[k][j] * rs;
-          const float n = hat * pw[k][j] + pb[k][j];
+          const float n = LAYER ? hat * pw[k][j] + pb[k][j] : hat * pw[k][j];
           float dn = u;
           dg[j] = u * n;
           if constexpr (GROUP) {
@@ -751,9 +796,12 @@ void launch_residual_norm_fwd(const ResidualNormParams& p, hipStream_t s) {
   check(p);
   if (p.P == 0) return;
   const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
-  const int blocks = fwd_blocks(p.P, p.C <= 512 ? 256 / narrow_lanes(p.C) : 1);
-  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((fwd_kernel<DT, LPR, WIDE, K>), dim3(blocks), dim3(threads),
-                                                             0, s, p, big(p, 4))));
+  const int blocks = fwd_blocks(p), nt = big(p, 4);
+#define DTF_FWD(LAYER)                                                                                         \
+  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((fwd_kernel<DT, LPR, WIDE, K, LAYER>), dim3(blocks), \
+                                                             dim3(threads), 0, s, p, nt)))
+  if (p.layer) { DTF_FWD(true); } else { DTF_FWD(false); }
+#undef DTF_FWD
 }
 
 void launch_residual_norm_bwd(const ResidualNormParams& p, hipStream_t s) {
