@@ -860,30 +860,28 @@ PYBIND11_MODULE(_dtf_native, m) {
   });
   m.attr("RESIDUAL_NORM_MAX_C") = RESIDUAL_NORM_MAX_C;
   py::class_<ClipList>(m, "ClipList")
-      .def(py::init([](const std::vector<uintptr_t>& in, const std::vector<uintptr_t>& out,
-                       const std::vector<int64_t>& n, const std::vector<int>& dt) {
-             if (n.size() != in.size() || dt.size() != in.size() || (!out.empty() && out.size() != in.size()))
-               throw std::invalid_argument("ClipList: lists of different lengths");
-             std::vector<ClipTensor> t(in.size());
-             for (size_t i = 0; i < in.size(); ++i)
-               t[i] = ClipTensor{reinterpret_cast<const void*>(in[i]),
-                                 out.empty() ? nullptr : reinterpret_cast<void*>(out[i]), n[i], dt[i]};
-             return new ClipList(t);
-           }), py::arg("in"), py::arg("out"), py::arg("n"), py::arg("dt"))
+      .def(py::init<const std::vector<uintptr_t>&, const std::vector<uintptr_t>&, const std::vector<int64_t>&,
+                    const std::vector<int>&>(), py::arg("in"), py::arg("out"), py::arg("n"), py::arg("dt"))
+      .def("table", [](const ClipList& l) { return py::bytes(l.table()); },
+           "What `resident` points to in device memory; empty where the arguments of one launch hold the list")
       .def_property_readonly("workspace_doubles", &ClipList::workspace_doubles)
-      .def("global_norm", [](const ClipList& l, uintptr_t ws, uintptr_t norm, uintptr_t s) {
+      .def("global_norm", [](const ClipList& l, uintptr_t resident, uintptr_t ws, uintptr_t norm, uintptr_t stream) {
              auto* w = reinterpret_cast<double*>(ws);
-             l.norm(w, reinterpret_cast<hipStream_t>(s));
-             l.finish(w, reinterpret_cast<float*>(norm), reinterpret_cast<hipStream_t>(s));
+             auto* r = reinterpret_cast<const void*>(resident);
+             auto s = reinterpret_cast<hipStream_t>(stream);
+             l.norm(r, w, s);
+             l.finish(r, w, reinterpret_cast<float*>(norm), s);
              check_launch(); },
-           py::arg("ws"), py::arg("norm"), py::arg("stream"))
-      .def("clip", [](const ClipList& l, uintptr_t ws, uintptr_t use_norm, float clip, uintptr_t norm, uintptr_t s) {
+           py::arg("resident"), py::arg("ws"), py::arg("norm"), py::arg("stream"))
+      .def("clip", [](const ClipList& l, uintptr_t resident, uintptr_t ws, uintptr_t use_norm, float clip, uintptr_t norm,
+                      uintptr_t stream) {
              auto* w = reinterpret_cast<double*>(ws);
-             if (!use_norm) l.norm(w, reinterpret_cast<hipStream_t>(s));
-             l.scale(w, reinterpret_cast<const float*>(use_norm), clip, reinterpret_cast<float*>(norm),
-                     reinterpret_cast<hipStream_t>(s));
+             auto* r = reinterpret_cast<const void*>(resident);
+             auto s = reinterpret_cast<hipStream_t>(stream);
+             if (!use_norm) l.norm(r, w, s);
+             l.scale(r, w, reinterpret_cast<const float*>(use_norm), clip, reinterpret_cast<float*>(norm), s);
              check_launch(); },
-           py::arg("ws"), py::arg("use_norm"), py::arg("clip"), py::arg("norm"), py::arg("stream"));
+           py::arg("resident"), py::arg("ws"), py::arg("use_norm"), py::arg("clip"), py::arg("norm"), py::arg("stream"));
   m.attr("PACK_PER_BLOCK") = 256 * 8;
   m.attr("arch") = "gfx950";
   py::class_<Plan>(m, "Plan")

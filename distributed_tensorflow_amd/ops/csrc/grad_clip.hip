@@ -13,8 +13,12 @@
 // A norm that is infinite or NaN makes every result NaN, as TensorFlow's clip_by_global_norm has it; a norm of zero
 // leaves the gradients alone.
 //
-// Tensors come as a table in the kernel's arguments: nothing to upload and keep alive, and a captured launch holds
-// its own copy.  The list is cut into chunks of 16 KB that never cross a tensor; a block takes a run of consecutive chunks.
+// Tensors are cut into chunks of 16 KB that never cross a tensor; the blocks walk the chunks side by side, two blocks
+// a CU (a narrow front over the memory: a read of 411 MB runs at 7.2 TB/s with 512 blocks, at 5.9 with 2048).  Which
+// tensor a chunk belongs to is looked up while the chunk before it is loaded: in a table in the kernel's arguments (a
+// list given as such: nothing to upload and keep alive, and a captured launch holds its own copy), or in device memory
+// (a table that is kept: any number of tensors in one launch).
+#include <algorithm>
 #include <stdexcept>
 
 #include "grad_clip.h"
@@ -23,14 +27,13 @@ namespace {
 
 constexpr int TPB = 256;
 constexpr int CHUNK_BYTES = TPB * 16 * 4;
-constexpr int MAX_BLOCKS = 2048;      // per launch: eight blocks a CU, all its waves
+constexpr int MAX_BLOCKS = 512;                    // per launch: two a CU
+constexpr int64_t CACHE_BYTES = 192 << 20;         // of what a sweep leaves in the memory-side cache (256 MB)
 
-struct __attribute__((packed, aligned(2))) Any16 { u32x4 v; };
-
-template <int DT> struct Vec { static constexpr int N = DT == DT_F32 ? 4 : 8; };
+typedef u32x4 __attribute__((aligned(2))) Any16;   // any address will do
 
 template <int DT>
-__device__ __forceinline__ void unpack(const u32x4 v, float* f) {
+__device__ __forceinline__ int unpack(const u32x4 v, float* f) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -41,16 +44,21 @@ __device__ __forceinline__ void unpack(const u32x4 v, float* f) {
       f[2 * j + 1] = hi16<DT>(w[j]);
     }
   }
+  return DT == DT_F32 ? 4 : 8;
 }
 template <int DT>
-__device__ __forceinline__ u32x4 pack(const float* f) {
-  u32x4 v;
+__device__ __forceinline__ u32x4 scaled(const u32x4 v, float factor) {
+  float f[8];
+  unpack<DT>(v, f);
+  u32x4 o;
   if constexpr (DT == DT_F32) {
-    v.x = __float_as_uint(f[0]); v.y = __float_as_uint(f[1]); v.z = __float_as_uint(f[2]); v.w = __float_as_uint(f[3]);
+    o.x = __float_as_uint(f[0] * factor); o.y = __float_as_uint(f[1] * factor);
+    o.z = __float_as_uint(f[2] * factor); o.w = __float_as_uint(f[3] * factor);
   } else {
-    v.x = pack2<DT>(f[0], f[1]); v.y = pack2<DT>(f[2], f[3]); v.z = pack2<DT>(f[4], f[5]); v.w = pack2<DT>(f[6], f[7]);
+    o.x = pack2<DT>(f[0] * factor, f[1] * factor); o.y = pack2<DT>(f[2] * factor, f[3] * factor);
+    o.z = pack2<DT>(f[4] * factor, f[5] * factor); o.w = pack2<DT>(f[6] * factor, f[7] * factor);
   }
-  return v;
+  return o;
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -83,92 +91,108 @@ __device__ __forceinline__ float clip_factor(const double* ws, int partials, con
   return norm > (double)clip ? (float)((double)clip / norm) : 1.f;
 }
 
-// The tensor that chunk `c` lies in.
-__device__ __forceinline__ int find(const ClipList::Table& t, uint32_t c) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.first[mid] <= c) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-template <int DT>
-__device__ __forceinline__ double chunk_squares(const void* in, int64_t n, uint32_t chunk) {
-  typedef typename Elem<DT>::T T;
-  constexpr int V = Vec<DT>::N;
-  const int64_t at = (int64_t)chunk * (TPB * 4 * V) + (int64_t)threadIdx.x * V;
-  const T* p = reinterpret_cast<const T*>(in);
-  float f[4][V];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int64_t e = at + (int64_t)k * TPB * V;
-    if (e + V <= n) {
-      unpack<DT>(reinterpret_cast<const Any16*>(p + e)->v, f[k]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) f[k][j] = e + j < n ? to_f<DT>(p[e + j]) : 0.f;
+struct Inline {         // a table in the arguments
+  ClipList::Table t;
+  __device__ __forceinline__ uint32_t chunks() const { return t.chunks; }
+  __device__ __forceinline__ ClipEntry at(uint32_t c) const {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t.e[mid].first <= c) lo = mid; else hi = mid - 1;
     }
+    return t.e[lo];
   }
-  double s[2] = {0., 0.};
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[j & 1] = fma((double)f[k][j], (double)f[k][j], s[j & 1]);
-  return s[0] + s[1];
-}
+};
+struct Resident {       // a table in device memory
+  const ClipEntry* e;
+  const uint32_t* map;
+  uint32_t n;
+  __device__ __forceinline__ uint32_t chunks() const { return n; }
+  __device__ __forceinline__ ClipEntry at(uint32_t c) const { return e[map[c]]; }
+};
 
-template <int DT>
-__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t n, uint32_t chunk, float factor) {
-  typedef typename Elem<DT>::T T;
-  constexpr int V = Vec<DT>::N;
-  const int64_t at = (int64_t)chunk * (TPB * 4 * V) + (int64_t)threadIdx.x * V;
-  const T* p = reinterpret_cast<const T*>(in);
-  T* q = reinterpret_cast<T*>(out);
-  u32x4 raw[4];
+// A thread's four pieces of 16 bytes of a chunk; past the tensor's end: zeros.
+template <bool NT>
+__device__ __forceinline__ void load_chunk(const ClipEntry& e, uint32_t c, u32x4* v) {
+  const int64_t at = (int64_t)(c - e.first) * CHUNK_BYTES + (int64_t)threadIdx.x * 16;
+  const char* p = reinterpret_cast<const char*>(e.in);
+  if (at - (int64_t)threadIdx.x * 16 + CHUNK_BYTES <= e.bytes) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int64_t e = at + (int64_t)k * TPB * V;
-    if (e + V <= n) raw[k] = reinterpret_cast<const Any16*>(p + e)->v;
-  }
+    for (int k = 0; k < 4; ++k) {
+      const Any16* q = reinterpret_cast<const Any16*>(p + at + k * TPB * 16);
+      if constexpr (NT) v[k] = __builtin_nontemporal_load(q);
+      else v[k] = *q;
+    }
+  } else {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int64_t e = at + (int64_t)k * TPB * V;
-    if (e + V <= n) {
-      float f[V];
-      unpack<DT>(raw[k], f);
+    for (int k = 0; k < 4; ++k) {
+      const int64_t o = at + k * TPB * 16;
+      v[k] = u32x4{0u, 0u, 0u, 0u};
+      if (o + 16 <= e.bytes) {
+        v[k] = *reinterpret_cast<const Any16*>(p + o);
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] *= factor;
-      reinterpret_cast<Any16*>(q + e)->v = pack<DT>(f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (e + j < n) q[e + j] = from_f<DT>(to_f<DT>(p[e + j]) * factor);
+        for (int j = 0; j < 8; ++j)
+          if (o + 2 * j < e.bytes) v[k][j >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p + o + 2 * j) << (16 * (j & 1));
+      }
     }
   }
 }
 
-constexpr int DT_SHIFT = 60;
+template <bool NT>
+__device__ __forceinline__ void store_chunk(const ClipEntry& e, uint32_t c, const u32x4* v) {
+  const int64_t at = (int64_t)(c - e.first) * CHUNK_BYTES + (int64_t)threadIdx.x * 16;
+  char* p = reinterpret_cast<char*>(e.out);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t o = at + k * TPB * 16;
+    if (o + 16 <= e.bytes) {
+      Any16* q = reinterpret_cast<Any16*>(p + o);
+      if constexpr (NT) __builtin_nontemporal_store((Any16)v[k], q);
+      else *q = v[k];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (o + 2 * j < e.bytes) *reinterpret_cast<uint16_t*>(p + o + 2 * j) = (uint16_t)(v[k][j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
 
-__global__ __launch_bounds__(TPB) void norm_kernel(const ClipList::Table t, double* __restrict__ ws) {
+template <int DT>
+__device__ __forceinline__ void add_squares(const u32x4* v, double* s) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float f[8];
+    const int n = unpack<DT>(v[k], f);
+#pragma unroll
+    for (int j = 0; j < n; ++j) s[j & 3] = fma((double)f[j], (double)f[j], s[j & 3]);
+  }
+}
+
+// Chunks before `cold` go past the caches: the sweep leaves the list's end there, where the scaling begins.
+template <typename T>
+__global__ __launch_bounds__(TPB) void norm_kernel(const T t, uint32_t cold, double* __restrict__ ws) {
   __shared__ double red[4];
-  const uint32_t chunks = t.first[t.count];
-  const uint32_t c0 = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x);
-  const uint32_t c1 = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
-  double s = 0.;
-  int i = c0 < c1 ? find(t, c0) : 0;
-  for (uint32_t c = c0; c < c1; ++c) {
-    while (c >= t.first[i + 1]) ++i;
-    const int64_t tag = t.n[i], n = tag & ((1ll << DT_SHIFT) - 1);
-    const uint32_t k = c - t.first[i];
-    switch ((int)(tag >> DT_SHIFT)) {
-      case DT_BF16: s += chunk_squares<DT_BF16>(t.in[i], n, k); break;
-      case DT_F16: s += chunk_squares<DT_F16>(t.in[i], n, k); break;
-      default: s += chunk_squares<DT_F32>(t.in[i], n, k); break;
+  double s[4] = {0., 0., 0., 0.};
+  const uint32_t chunks = t.chunks();
+  uint32_t c = blockIdx.x;
+  ClipEntry e = {};
+  if (c < chunks) e = t.at(c);
+  while (c < chunks) {
+    u32x4 v[4];
+    if (c < cold) load_chunk<true>(e, c, v);
+    else load_chunk<false>(e, c, v);
+    const int dt = e.dt;
+    c += gridDim.x;
+    if (c < chunks) e = t.at(c);
+    switch (dt) {
+      case DT_BF16: add_squares<DT_BF16>(v, s); break;
+      case DT_F16: add_squares<DT_F16>(v, s); break;
+      default: add_squares<DT_F32>(v, s); break;
     }
   }
-  s = block_sum64(s, red);
-  if (threadIdx.x == 0) ws[blockIdx.x] = s;
+  const double sum = block_sum64((s[0] + s[1]) + (s[2] + s[3]), red);
+  if (threadIdx.x == 0) ws[blockIdx.x] = sum;
 }
 
 __global__ __launch_bounds__(TPB) void norm_finish_kernel(const double* __restrict__ ws, int partials, float* norm) {
@@ -176,25 +200,30 @@ __global__ __launch_bounds__(TPB) void norm_finish_kernel(const double* __restri
   (void)clip_factor(ws, partials, nullptr, 1.f, norm, red);
 }
 
-__global__ __launch_bounds__(TPB) void scale_kernel(const ClipList::Table t, const double* __restrict__ ws,
-                                                    int partials, const float* __restrict__ use_norm, float clip,
-                                                    float* norm, int in_place) {
+template <typename T>
+__global__ __launch_bounds__(TPB) void scale_kernel(const T t, const double* __restrict__ ws, int partials,
+                                                    const float* __restrict__ use_norm, float clip, float* norm,
+                                                    int in_place, int nt) {
   __shared__ double red[4];
   const float factor = clip_factor(ws, partials, use_norm, clip, norm, red);
   if (in_place && factor == 1.f) return;        // every result is where it belongs already
-  const uint32_t chunks = t.first[t.count], b = gridDim.x - 1 - blockIdx.x;
-  const uint32_t c0 = (uint32_t)((uint64_t)chunks * b / gridDim.x);
-  const uint32_t c1 = (uint32_t)((uint64_t)chunks * (b + 1) / gridDim.x);
-  int i = c0 < c1 ? find(t, c1 - 1) : 0;
-  for (uint32_t c = c1; c-- > c0;) {
-    while (c < t.first[i]) --i;
-    const int64_t tag = t.n[i], n = tag & ((1ll << DT_SHIFT) - 1);
-    const uint32_t k = c - t.first[i];
-    switch ((int)(tag >> DT_SHIFT)) {
-      case DT_BF16: chunk_scale<DT_BF16>(t.in[i], t.out[i], n, k, factor); break;
-      case DT_F16: chunk_scale<DT_F16>(t.in[i], t.out[i], n, k, factor); break;
-      default: chunk_scale<DT_F32>(t.in[i], t.out[i], n, k, factor); break;
-    }
+  const uint32_t chunks = t.chunks();
+  uint32_t k = blockIdx.x;                      // from the end, which the norm's sweep has left in the cache
+  ClipEntry next = {};
+  if (k < chunks) next = t.at(chunks - 1 - k);
+  while (k < chunks) {
+    const ClipEntry e = next;
+    const uint32_t c = chunks - 1 - k;
+    u32x4 v[4];
+    load_chunk<false>(e, c, v);
+    k += gridDim.x;
+    if (k < chunks) next = t.at(chunks - 1 - k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = e.dt == DT_BF16 ? scaled<DT_BF16>(v[i], factor) : e.dt == DT_F16 ? scaled<DT_F16>(v[i], factor)
+                                                                               : scaled<DT_F32>(v[i], factor);
+    if (nt) store_chunk<true>(e, c, v);
+    else store_chunk<false>(e, c, v);
   }
 }
 
@@ -208,7 +237,7 @@ __device__ __forceinline__ void unscale(const float* skip, float* grad_scale) {
 
 __global__ __launch_bounds__(TPB) void sgd_norm_kernel(const float* __restrict__ p, const float* __restrict__ g,
                                                        const float* __restrict__ l2x2, size_t n, float grad_scale,
-                                                       const float* __restrict__ skip, double* __restrict__ ws) {
+                                                       const float* __restrict__ skip, size_t cold, double* __restrict__ ws) {
   __shared__ double red[4];
   unscale(skip, &grad_scale);
   const size_t n4 = n / 4, stride = (size_t)gridDim.x * TPB;
@@ -223,11 +252,20 @@ __global__ __launch_bounds__(TPB) void sgd_norm_kernel(const float* __restrict__
   size_t i = blockIdx.x * (size_t)TPB + threadIdx.x;
   for (; i + 3 * stride < n4; i += 4 * stride) {       // twelve loads under way
     f32x4 w[4], gr[4], l2[4];
+    if (i + 3 * stride < cold) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = reinterpret_cast<const f32x4*>(p)[i + k * stride];
-      gr[k] = reinterpret_cast<const f32x4*>(g)[i + k * stride];
-      l2[k] = reinterpret_cast<const f32x4*>(l2x2)[i + k * stride];
+      for (int k = 0; k < 4; ++k) {
+        w[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p) + i + k * stride);
+        gr[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(g) + i + k * stride);
+        l2[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(l2x2) + i + k * stride);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k] = reinterpret_cast<const f32x4*>(p)[i + k * stride];
+        gr[k] = reinterpret_cast<const f32x4*>(g)[i + k * stride];
+        l2[k] = reinterpret_cast<const f32x4*>(l2x2)[i + k * stride];
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) take(w[k], gr[k], l2[k]);
@@ -243,18 +281,51 @@ __global__ __launch_bounds__(TPB) void sgd_norm_kernel(const float* __restrict__
   if (threadIdx.x == 0) ws[blockIdx.x] = sum;
 }
 
+template <bool NT, int U>
+__device__ __forceinline__ void update(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ v,
+                                       const float* __restrict__ l2x2, size_t at, size_t stride, float momentum,
+                                       float grad_scale, float step) {
+  f32x4 w[U], gr[U], l2[U], vel[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const size_t i = at - k * stride;
+    w[k] = reinterpret_cast<const f32x4*>(p)[i];
+    gr[k] = reinterpret_cast<const f32x4*>(g)[i];
+    l2[k] = reinterpret_cast<const f32x4*>(l2x2)[i];
+    if (momentum != 0.f) {
+      if constexpr (NT) vel[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(v) + i);
+      else vel[k] = reinterpret_cast<const f32x4*>(v)[i];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const size_t i = at - k * stride;
+    const f32x4 d = gr[k] * grad_scale + l2[k] * w[k];
+    if (momentum != 0.f) {
+      vel[k] = vel[k] * momentum - d * step;
+      w[k] += vel[k];
+      if constexpr (NT) __builtin_nontemporal_store(vel[k], reinterpret_cast<f32x4*>(v) + i);
+      else reinterpret_cast<f32x4*>(v)[i] = vel[k];
+    } else {
+      w[k] -= d * step;
+    }
+    if constexpr (NT) __builtin_nontemporal_store(w[k], reinterpret_cast<f32x4*>(p) + i);
+    else reinterpret_cast<f32x4*>(p)[i] = w[k];
+  }
+}
+
 __global__ __launch_bounds__(TPB) void clipped_sgd_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                           float* __restrict__ v, const float* __restrict__ l2x2,
                                                           size_t n, float lr, float momentum, float grad_scale,
                                                           float clip, const float* __restrict__ skip,
-                                                          const double* __restrict__ ws, int partials, float* norm) {
+                                                          const double* __restrict__ ws, int partials, float* norm,
+                                                          int nt) {
   __shared__ double red[4];
   unscale(skip, &grad_scale);
   const float factor = clip_factor(ws, partials, nullptr, clip, norm, red);
   if (skip && skip[0] != 0.f) return;       // a gradient is not finite: the step is left out
   const float step = lr * factor;
   const size_t n4 = n / 4, stride = (size_t)gridDim.x * TPB;
-  const size_t first = blockIdx.x * (size_t)TPB + threadIdx.x;
   if (blockIdx.x == 0 && n4 * 4 + threadIdx.x < n) {
     const size_t t = n4 * 4 + threadIdx.x;
     const float w = p[t], d = g[t] * grad_scale + l2x2[t] * w;
@@ -262,89 +333,127 @@ __global__ __launch_bounds__(TPB) void clipped_sgd_kernel(float* __restrict__ p,
     if (momentum != 0.f) { vel = v[t] * momentum - d * step; v[t] = vel; }
     p[t] = w + vel;
   }
-  for (size_t k = first; k < n4; k += stride) {
-    const size_t i = n4 - 1 - k;
-    f32x4 w = reinterpret_cast<const f32x4*>(p)[i];
-    const f32x4 gr = reinterpret_cast<const f32x4*>(g)[i], l2 = reinterpret_cast<const f32x4*>(l2x2)[i];
-    const f32x4 d = gr * grad_scale + l2 * w;
-    if (momentum != 0.f) {
-      f32x4 vel = reinterpret_cast<const f32x4*>(v)[i];
-      vel = vel * momentum - d * step;
-      reinterpret_cast<f32x4*>(v)[i] = vel;
-      w += vel;
-    } else {
-      w -= d * step;
-    }
-    reinterpret_cast<f32x4*>(p)[i] = w;
+  // from the end, which the norm's sweep has left in the cache
+  size_t k = blockIdx.x * (size_t)TPB + threadIdx.x;
+  for (; k + 3 * stride < n4; k += 4 * stride) {
+    if (nt) update<true, 4>(p, g, v, l2x2, n4 - 1 - k, stride, momentum, grad_scale, step);
+    else update<false, 4>(p, g, v, l2x2, n4 - 1 - k, stride, momentum, grad_scale, step);
   }
+  for (; k < n4; k += stride) update<false, 1>(p, g, v, l2x2, n4 - 1 - k, stride, momentum, grad_scale, step);
 }
 
 int elem_bytes(int dt) { return dt == DT_F32 ? 4 : 2; }
 
 }  // namespace
 
-ClipList::ClipList(const std::vector<ClipTensor>& tensors) {
-  size_t i = 0;
-  while (i < tensors.size()) {
+ClipList::ClipList(const std::vector<uintptr_t>& in, const std::vector<uintptr_t>& out, const std::vector<int64_t>& n,
+                   const std::vector<int>& dt) {
+  if (n.size() != in.size() || dt.size() != in.size() || (!out.empty() && out.size() != in.size()))
+    throw std::invalid_argument("ClipList: lists of different lengths");
+  for (size_t i = 0; i < in.size(); ++i) {
+    if (dt[i] != DT_BF16 && dt[i] != DT_F16 && dt[i] != DT_F32) throw std::invalid_argument("unknown element type");
+    if (n[i] < 0 || n[i] >= (1ll << 40)) throw std::invalid_argument("a tensor of up to 2^40 elements");
+    if (n[i] == 0) continue;
+    ClipEntry e;
+    e.in = reinterpret_cast<const void*>(in[i]);
+    e.out = out.empty() ? nullptr : reinterpret_cast<void*>(out[i]);
+    e.bytes = n[i] * elem_bytes(dt[i]);
+    e.dt = dt[i];
+    e.first = (uint32_t)chunks_;
+    chunks_ += ((uint64_t)e.bytes + CHUNK_BYTES - 1) / CHUNK_BYTES;
+    if (chunks_ > 0x7fffffffull) throw std::invalid_argument("a list of up to 32 TB");
+    bytes_ += e.bytes;
+    in_place_ = in_place_ && e.in == e.out;
+    outputs_ = outputs_ && e.out;
+    all_.push_back(e);
+  }
+  for (size_t i = 0; i < all_.size(); i += PER_LAUNCH) {
     Piece piece;
     Table& t = piece.table;
     t = Table();
-    uint64_t chunks = 0;
-    for (; i < tensors.size() && t.count < PER_LAUNCH; ++i) {
-      const ClipTensor& x = tensors[i];
-      if (x.dt != DT_BF16 && x.dt != DT_F16 && x.dt != DT_F32) throw std::invalid_argument("unknown element type");
-      if (x.n < 0 || x.n >= (1ll << 40)) throw std::invalid_argument("a tensor of up to 2^40 elements");
-      if (x.n == 0) continue;
-      const uint64_t mine = ((uint64_t)x.n * elem_bytes(x.dt) + CHUNK_BYTES - 1) / CHUNK_BYTES;
-      if (chunks + mine > 0xfffffff0ull) {
-        if (t.count == 0) throw std::invalid_argument("a tensor is too large");
-        break;
-      }
-      t.in[t.count] = x.in;
-      t.out[t.count] = x.out;
-      t.n[t.count] = x.n | ((int64_t)x.dt << DT_SHIFT);
-      t.first[t.count] = (uint32_t)chunks;
-      chunks += mine;
-      ++t.count;
+    t.count = (int)std::min<size_t>(PER_LAUNCH, all_.size() - i);
+    for (int k = 0; k < t.count; ++k) {
+      t.e[k] = all_[i + k];
+      t.e[k].first -= all_[i].first;
     }
-    if (t.count == 0) continue;
-    t.first[t.count] = (uint32_t)chunks;
-    piece.blocks = (int)(chunks < (uint64_t)MAX_BLOCKS ? chunks : (uint64_t)MAX_BLOCKS);
+    t.chunks = (uint32_t)((i + t.count < all_.size() ? all_[i + t.count].first : chunks_) - all_[i].first);
     piece.at = partials_;
-    partials_ += piece.blocks;
+    partials_ += std::min<uint32_t>(t.chunks, MAX_BLOCKS);
     pieces_.push_back(piece);
   }
 }
 
-void ClipList::norm(double* ws, hipStream_t s) const {
-  for (const Piece& p : pieces_)
-    hipLaunchKernelGGL(norm_kernel, dim3(p.blocks), dim3(TPB), 0, s, p.table, ws + p.at);
+std::string ClipList::table() const {
+  if (pieces_.size() < 2) return std::string();
+  std::string s(reinterpret_cast<const char*>(all_.data()), all_.size() * sizeof(ClipEntry));
+  std::vector<uint32_t> map(chunks_);
+  for (size_t i = 0; i < all_.size(); ++i)
+    std::fill(map.begin() + all_[i].first, i + 1 < all_.size() ? map.begin() + all_[i + 1].first : map.end(), (uint32_t)i);
+  return s + std::string(reinterpret_cast<const char*>(map.data()), map.size() * sizeof(uint32_t));
 }
 
-void ClipList::finish(const double* ws, float* norm, hipStream_t s) const {
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(TPB), 0, s, ws, (int)partials_, norm);
+namespace {
+
+Resident resident_table(const void* at, size_t entries, uint64_t chunks) {
+  Resident r;
+  r.e = reinterpret_cast<const ClipEntry*>(at);
+  r.map = reinterpret_cast<const uint32_t*>(r.e + entries);
+  r.n = (uint32_t)chunks;
+  return r;
+}
+int list_blocks(uint64_t chunks) { return (int)std::min<uint64_t>(chunks, MAX_BLOCKS); }
+
+}  // namespace
+
+void ClipList::norm(const void* resident, double* ws, hipStream_t s) const {
+  // a list that the cache holds is read through it; of a larger one, the end is
+  const uint32_t cold = bytes_ <= CACHE_BYTES ? 0 : (uint32_t)((bytes_ - CACHE_BYTES) / CHUNK_BYTES);
+  if (resident) {
+    hipLaunchKernelGGL(norm_kernel<Resident>, dim3(list_blocks(chunks_)), dim3(TPB), 0, s,
+                       resident_table(resident, all_.size(), chunks_), cold, ws);
+    return;
+  }
+  uint64_t before = 0;
+  for (const Piece& p : pieces_) {
+    const uint32_t c = cold > before ? (uint32_t)(cold - before) : 0;
+    hipLaunchKernelGGL(norm_kernel<Inline>, dim3(list_blocks(p.table.chunks)), dim3(TPB), 0, s, Inline{p.table}, c,
+                       ws + p.at);
+    before += p.table.chunks;
+  }
 }
 
-void ClipList::scale(const double* ws, const float* use_norm, float clip, float* norm, hipStream_t s) const {
-  if (pieces_.empty()) {
-    if (!use_norm) finish(ws, norm, s);
+int ClipList::partials(const void* resident) const { return resident ? list_blocks(chunks_) : (int)partials_; }
+
+void ClipList::finish(const void* resident, const double* ws, float* norm, hipStream_t s) const {
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(TPB), 0, s, ws, partials(resident), norm);
+}
+
+void ClipList::scale(const void* resident, const double* ws, const float* use_norm, float clip, float* norm,
+                     hipStream_t s) const {
+  if (!(clip > 0.f)) throw std::invalid_argument("clip: the clip norm has to be positive");
+  if (all_.empty()) {
+    if (!use_norm) finish(resident, ws, norm, s);
+    return;
+  }
+  if (!outputs_) throw std::invalid_argument("clip: a list without outputs");
+  // results that would drive the rest of the list out of the cache go past it
+  const int nt = 2 * bytes_ > CACHE_BYTES;
+  const int count = partials(resident);
+  if (resident) {
+    hipLaunchKernelGGL(scale_kernel<Resident>, dim3(list_blocks(chunks_)), dim3(TPB), 0, s,
+                       resident_table(resident, all_.size(), chunks_), ws, count, use_norm, clip, norm, (int)in_place_, nt);
     return;
   }
   for (size_t k = pieces_.size(); k-- > 0;) {
     const Piece& p = pieces_[k];
-    bool in_place = true;
-    for (int i = 0; i < p.table.count; ++i) {
-      if (!p.table.out[i]) throw std::invalid_argument("clip: a list without outputs");
-      in_place = in_place && p.table.out[i] == p.table.in[i];
-    }
-    hipLaunchKernelGGL(scale_kernel, dim3(p.blocks), dim3(TPB), 0, s, p.table, ws, (int)partials_, use_norm, clip,
-                       k + 1 == pieces_.size() ? norm : (float*)nullptr, (int)in_place);
+    hipLaunchKernelGGL(scale_kernel<Inline>, dim3(list_blocks(p.table.chunks)), dim3(TPB), 0, s, Inline{p.table}, ws,
+                       count, use_norm, clip, k + 1 == pieces_.size() ? norm : (float*)nullptr, (int)in_place_, nt);
   }
 }
 
 int clipped_sgd_blocks(size_t n) {
   const size_t want = (n / 4 + TPB - 1) / TPB;
-  return (int)(want < 1 ? 1 : want < 1024 ? want : 1024);
+  return (int)std::min<size_t>(std::max<size_t>(want, 1), MAX_BLOCKS);
 }
 
 void launch_clipped_sgd_momentum_l2(float* p, const float* g, float* v, const float* l2x2, size_t n, float lr,
@@ -353,10 +462,10 @@ void launch_clipped_sgd_momentum_l2(float* p, const float* g, float* v, const fl
   if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)v | (uintptr_t)l2x2) & 15)
     throw std::invalid_argument("clipped sgd: buffers must be 16-byte aligned");
   if (!(clip > 0.f)) throw std::invalid_argument("clipped sgd: the clip norm has to be positive");
-  const int partials = clipped_sgd_blocks(n);
-  hipLaunchKernelGGL(sgd_norm_kernel, dim3(partials), dim3(TPB), 0, s, p, g, l2x2, n, grad_scale, skip, ws);
-  const size_t want = (n / 4 + TPB - 1) / TPB;
-  const int blocks = (int)(want < 1 ? 1 : want < 2048 ? want : 2048);
+  const int blocks = clipped_sgd_blocks(n);
+  // three buffers are read for the norm: what of them the cache can keep for the update is read through it
+  const size_t keep = CACHE_BYTES / 48, n4 = n / 4, cold = n4 > keep ? n4 - keep : 0;
+  hipLaunchKernelGGL(sgd_norm_kernel, dim3(blocks), dim3(TPB), 0, s, p, g, l2x2, n, grad_scale, skip, cold, ws);
   hipLaunchKernelGGL(clipped_sgd_kernel, dim3(blocks), dim3(TPB), 0, s, p, g, v, l2x2, n, lr, momentum, grad_scale,
-                     clip, skip, ws, partials, norm);
+                     clip, skip, ws, blocks, norm, (int)(n4 * 96 > (size_t)CACHE_BYTES));
 }

@@ -198,6 +198,7 @@ __device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, f
 template <int DT, int K>
 struct FwdIn {
   Raw8<DT> x[K], y[K], gate[K];
+  Raw8<DT_F32> group[K];
 };
 
 template <int DT, int K, bool NT>
@@ -209,12 +210,15 @@ __device__ __forceinline__ void load_fwd(FwdIn<DT, K>& in, const ResidualNormPar
     if (p.y) in.y[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
     if (p.gate_mode == GATE_ELEMENT)
       in.gate[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
+    if (p.gate_mode == GATE_GROUP)
+      in.group[k] = load_raw<DT_F32>(reinterpret_cast<const float*>(p.gate) +
+                                         (int64_t)((uint32_t)r / (uint32_t)p.group_rows) * p.ldgate, c[k], C);
   }
 }
 
-// A block takes a run of consecutive rows: while one row's sums are taken the next one's loads are under way, the
-// vectors stay in registers, and a gate row is read again only where its group ends.
-// Waves per SIMD that its registers allow; the grid is what is resident at once.
+// The blocks walk the rows side by side: while one row's sums are taken the next one's loads are under way, and the
+// vectors stay in registers.
+// Waves per SIMD that the registers are kept small enough for.
 constexpr int fwd_waves(int dt, bool layer, int chunks) { return chunks > 1 ? 2 : layer && dt == DT_F32 ? 3 : 4; }
 
 template <int DT, int LPR, bool WIDE, int K, bool LAYER>
@@ -243,43 +247,30 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, fwd_waves(DT, LAYER, K)) void fwd
   }
   // every lane of a wave walks the same number of passes (the sums need all of them); a row past the run's end has
   // no channels: zeros are read and nothing is written for it
-  const int64_t row0 = (int64_t)p.P * blockIdx.x / gridDim.x, row1 = (int64_t)p.P * (blockIdx.x + 1) / gridDim.x;
+  const int64_t row0 = (int64_t)blockIdx.x * slots, row1 = p.P, step = (int64_t)gridDim.x * slots;
   FwdIn<DT, K> next;
-  auto ask = [&](int64_t row) {
-    const int Cr = row < row1 ? C : 0;
-    const int64_t r = row < row1 ? row : 0;
+  auto ask = [&](int64_t base) {
+    if (base >= row1) return;
+    const int Cr = base + slot < row1 ? C : 0;
+    const int64_t r = base + slot < row1 ? base + slot : 0;
     if (nt) load_fwd<DT, K, true>(next, p, r, c, Cr);
     else load_fwd<DT, K, false>(next, p, r, c, Cr);
   };
-  int group = -1;
-  if (row0 < row1) ask(row0 + slot);
-  for (int64_t base = row0; base < row1; base += slots) {
+  ask(row0);
+  for (int64_t base = row0; base < row1; base += step) {
     const FwdIn<DT, K> in = next;
     const int64_t r = base + slot < row1 ? base + slot : 0;
     const int Cr = base + slot < row1 ? C : 0;
-    if (base + slots < row1) ask(base + slots + slot);
+    ask(base + step);
     float h[K][8], v[K][8];
 #pragma unroll
     for (int k = 0; k < K; ++k) unpack8<DT>(in.x[k], h[k]);
     if (p.y) {
-      if (p.gate_mode == GATE_GROUP) {
-        const int now = (int)((uint32_t)r / (uint32_t)p.group_rows);
-        if (now != group) {
-          group = now;
-          const float* row_g = reinterpret_cast<const float*>(p.gate) + (int64_t)now * p.ldgate;
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            load8<DT_F32>(row_g, c[k], C, g[k]);
-            if (p.sigmoid) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
-            }
-          }
-        }
-      } else if (p.gate_mode == GATE_ELEMENT) {
+      if (p.gate_mode != GATE_NONE) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          unpack8<DT>(in.gate[k], g[k]);
+          if (p.gate_mode == GATE_GROUP) unpack8<DT_F32>(in.group[k], g[k]);
+          else unpack8<DT>(in.gate[k], g[k]);
           if (p.sigmoid) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
@@ -332,7 +323,6 @@ struct BwdPlan {
   int parts;         // blocks per group
   int groups;        // groups of rows (1 without a group gate)
   int group_rows;
-  int part_rows;     // rows of a group per part
   int own_groups;    // each row slot takes whole groups
   int nt;            // more bytes than the memory-side cache holds: loads and stores past the caches
 };
@@ -358,10 +348,14 @@ int big(const ResidualNormParams& p, int tensors) {
   return (int64_t)p.P * p.C * (p.dt == DT_F32 ? 4 : 2) * tensors > (256ll << 20);
 }
 
-int fwd_blocks(const ResidualNormParams& p) {
+// Sweeps over more than the cache holds run best as a narrow front: eight waves a CU and accesses past the caches
+// (200704 x 512 bf16 with a gate per image: 140 us; 158 with sixteen waves, 206 through the caches; the gradient with
+// a gate per element: 286; 312 with twelve).  What the cache holds wants every wave there is room for (4099 x 1001
+// fp16: 48, 27, 18, 14, 13 us with 2, 4, 8, 16, 32 waves a CU).
+int fwd_blocks(const ResidualNormParams& p, int nt) {
   const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
   const int waves = (p.C <= 512 ? 256 : wide_threads(p.C)) / 64;
-  const int most = 256 * std::max(1, 4 * fwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2) / waves);
+  const int most = 256 * std::max(1, (nt ? 8 : 32) / waves);
   const int64_t want = ((int64_t)p.P + slots - 1) / slots;
   return (int)(want < most ? want : most);
 }
@@ -373,26 +367,35 @@ BwdPlan plan_bwd(const ResidualNormParams& p) {
   b.groups = p.P / b.group_rows;
   const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
   const int waves = (p.C <= 512 ? 256 : wide_threads(p.C)) / 64;
-  const int want = 256 * max(1, 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2) / waves);
   b.nt = big(p, 6);
+  // the grid is what is resident at once: no half-empty second round of blocks
+  const int resident = 256 * std::max(1, 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2) / waves);
+  const int want = b.nt && !grouped ? std::min(resident, 256 * std::max(1, 8 / waves)) : resident;
   b.own_groups = grouped && slots > 1 && b.group_rows < 4 * slots;
   if (b.own_groups) {
     const int sets = (b.groups + slots - 1) / slots;
     b.blocks = sets < want ? sets : want;
     b.parts = 1;
-    b.part_rows = b.group_rows;
     return b;
   }
-  if (b.groups >= want) {
-    b.blocks = want;
-    b.parts = 1;
-  } else {
-    int most = (b.group_rows + slots - 1) / slots;         // a part has work for every slot
-    b.parts = want / b.groups;
-    if (b.parts > most) b.parts = most;
+  b.parts = 1;
+  if (b.groups == 1) {
+    b.parts = std::min((b.group_rows + slots - 1) / slots, want);      // a part has work for every slot
+    b.blocks = b.parts;
+  } else if (b.groups < 4 * want) {
+    // as many parts as leave the fewest rows to the busiest slot on the grid (a few percent are worth fewer partial sums)
+    const int most = std::min((b.group_rows + slots - 1) / slots, std::max(16, want / b.groups));
+    double best = 1e30;
+    for (int parts = 1; parts <= most; ++parts) {
+      const int64_t rounds = ((int64_t)b.groups * parts + want - 1) / want;
+      if (rounds > 1 && parts > 16) break;
+      const double rows = (double)rounds * ((b.group_rows + (int64_t)parts * slots - 1) / ((int64_t)parts * slots));
+      if (rows * (rounds > 1 ? 1.05 : 1.0) < 0.97 * best) { best = rows * (rounds > 1 ? 1.05 : 1.0); b.parts = parts; }
+    }
     b.blocks = b.groups * b.parts;
+  } else {
+    b.blocks = want;
   }
-  b.part_rows = (b.group_rows + b.parts - 1) / b.parts;
   return b;
 }
 
@@ -465,9 +468,9 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
   const int first_set = plan.parts > 1 ? (int)blockIdx.x / plan.parts : (int)blockIdx.x;
   const int stride_set = plan.parts > 1 ? plan.groups : (int)gridDim.x;      // parts > 1: one group a block
   const int sets = (plan.groups + per_set - 1) / per_set;
-  const int row0 = plan.parts > 1 ? ((int)blockIdx.x % plan.parts) * plan.part_rows : 0;
-  const int row1 = min(row0 + plan.part_rows, plan.group_rows);
-  const int step = plan.own_groups ? 1 : slots;
+  const int row0 = plan.parts > 1 ? ((int)blockIdx.x % plan.parts) * slots : 0;
+  const int row1 = plan.group_rows;
+  const int step = plan.own_groups ? 1 : slots * plan.parts;     // the blocks of a group walk its rows side by side
   for (int set = first_set; set < sets; set += stride_set) {
     const int group = plan.own_groups ? set * slots + slot : set;
     const bool group_live = group < plan.groups;
@@ -490,23 +493,21 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
       *r = live ? (int64_t)group * plan.group_rows + in_group : 0;
       return live ? C : 0;
     };
+    // the next row's loads are under way while this row's sums are taken
     RowIn<DT, K> next;
-    int64_t r_next = 0;
-    int C_next = 0;
-    if (row0 < row1) {
-      C_next = row_of(row0, &r_next);
-      if (nt) load_row<DT, K, true>(next, p, r_next, c, C_next);
-      else load_row<DT, K, false>(next, p, r_next, c, C_next);
-    }
+    auto ask = [&](int rr) {
+      if (rr >= row1) return;
+      int64_t r;
+      const int Cr = row_of(rr, &r);
+      if (nt) load_row<DT, K, true>(next, p, r, c, Cr);
+      else load_row<DT, K, false>(next, p, r, c, Cr);
+    };
+    ask(row0);
     for (int rr = row0; rr < row1; rr += step) {
       const RowIn<DT, K> in = next;
-      const int64_t r = r_next;
-      const int Cr = C_next;
-      if (rr + step < row1) {          // the next row's loads are under way while this row's sums are taken
-        C_next = row_of(rr + step, &r_next);
-        if (nt) load_row<DT, K, true>(next, p, r_next, c, C_next);
-        else load_row<DT, K, false>(next, p, r_next, c, C_next);
-      }
+      int64_t r;
+      const int Cr = row_of(rr, &r);
+      ask(rr + step);
       float up[K][8], h[K][8], v[K][8];
 #pragma unroll
       for (int k = 0; k < K; ++k) unpack8<DT>(in.dh[k], up[k]);
@@ -760,7 +761,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
 
 void check(const ResidualNormParams& p) {
   if (p.C < 1 || p.C > RESIDUAL_NORM_MAX_C) throw std::invalid_argument("residual_norm: 1 to 8192 channels");
-  if (p.P < 0 || p.P > 0x7fff0000) throw std::invalid_argument("residual_norm: too many rows");
+  if (p.P < 0 || p.P > 0x7ff00000) throw std::invalid_argument("residual_norm: too many rows");
   if (!(p.eps > 0.f)) throw std::invalid_argument("residual_norm: eps has to be positive");   // rows of zeros
   if (p.gate_mode == GATE_GROUP && (p.group_rows < 1 || p.P % p.group_rows))
     throw std::invalid_argument("residual_norm: the rows of a gate's groups have to divide the rows");
@@ -796,7 +797,7 @@ void launch_residual_norm_fwd(const ResidualNormParams& p, hipStream_t s) {
   check(p);
   if (p.P == 0) return;
   const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
-  const int blocks = fwd_blocks(p), nt = big(p, 4);
+  const int nt = big(p, 4), blocks = fwd_blocks(p, nt);
 #define DTF_FWD(LAYER)                                                                                         \
   DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((fwd_kernel<DT, LPR, WIDE, K, LAYER>), dim3(blocks), \
                                                              dim3(threads), 0, s, p, nt)))

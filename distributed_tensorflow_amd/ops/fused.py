@@ -279,11 +279,12 @@ class TensorTable:
 
   `out`: where clipped tensors go, a list of the same shapes and types (the tensors themselves: in place); without
   it they are clipped in place.  The table keeps the tensors alive and follows them: one whose storage was exchanged
-  since is looked up again by the next call.  Contiguous bfloat16, float16 or float32 tensors of one device; outputs may
+  since is looked up again by the next call.  Keep the table itself for as long as a graph that was captured with it.  Contiguous bfloat16, float16 or float32 tensors of one device; outputs may
   not overlap each other, nor any input but their own.
   """
 
-  def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
+  def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None, *, _kept=True):
+    self._kept = _kept
     self.tensors = list(tensors)
     self.out = self.tensors if out is None else list(out)
     if not self.tensors:
@@ -309,12 +310,11 @@ class TensorTable:
     outs = [_span(o) for o in self.out]
     apart = [_span(t) for t, o in zip(self.tensors, self.out) if t.data_ptr() != o.data_ptr()]
     self._clash = _overlaps(outs) or (bool(apart) and _overlaps_two(outs, apart))
-    self.list, self.workspace = None, 0        # native: the launches' tables, doubles they need
+    # native: the launches, the doubles they need, their table in device memory and the stream it was written on
+    self.list, self.workspace, self.resident, self.stream = None, 0, None, 0
     if self.device.type == "cuda":
       from . import native  # pylint: disable=import-outside-toplevel
-      self.list = native.ext().ClipList(self._at, self._to, [t.numel() for t in self.tensors],
-                                         [native.dtype_code(t.dtype) for t in self.tensors])
-      self.workspace = max(self.list.workspace_doubles, 1)
+      native.clip_list_build(self, self._at, self._to, self._kept)
 
   def _current(self) -> "TensorTable":
     if self._at != list(map(torch.Tensor.data_ptr, self.tensors)) or (
@@ -339,7 +339,7 @@ def _table(tensors) -> TensorTable:
     return tensors._current()
   if isinstance(tensors, torch.Tensor):
     raise ValueError("a list of tensors (or a TensorTable), not a tensor")
-  return TensorTable(tensors)
+  return TensorTable(tensors, _kept=False)
 
 
 def _squares(tensors) -> torch.Tensor:

@@ -18,7 +18,8 @@ except ImportError as e:                      # pragma: no cover - exercised onl
   _import_error = e
 
 __all__ = ["available", "ext", "run_op", "Plan", "stream_handle", "sgd_momentum_l2", "loss_scale_step",
-           "clipped_sgd_momentum_l2", "clip_list_norm", "clip_list_scale",
+           "clipped_sgd_momentum_l2", "clip_list_build", "clip_list_norm",
+           "clip_list_scale",
            "residual_norm", "residual_norm_grad", "dtype_code", "pack_desc_bytes", "pack_blocks", "PACK_PER_BLOCK"]
 
 PACK_PER_BLOCK = 256 * 8
@@ -102,15 +103,43 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
   return norm
 
 
+def clip_list_build(table, at: List[int], to: List[int], kept: bool):
+  """Native half of a `fused.TensorTable`.  One that is kept and does not fit the arguments of a launch gets a table in
+  device memory (not while a graph is captured: an upload would become part of it)."""
+  ts = table.tensors
+  table.list = ext().ClipList(at, to, [t.numel() for t in ts], [dtype_code(t.dtype) for t in ts])
+  table.workspace = max(table.list.workspace_doubles, 1)
+  if kept and not torch.cuda.is_current_stream_capturing():
+    raw = table.list.table()
+    if raw:
+      with torch.cuda.device(table.device):
+        # a blocking copy: complete for every stream when it returns
+        table.resident = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(table.device)
+        table.stream = _current_stream(table.device.index)
+
+
+def _clip_list_launch(table, stream: int):
+  """(address of the device table or 0, norm, workspace) of a call.  The workspace is the call's own: tables are shared
+  between streams.  The device table is held back from reuse until a foreign stream is done with it."""
+  dev = table.device
+  resident = 0
+  if table.resident is not None:
+    resident = table.resident.data_ptr()
+    if stream != table.stream:
+      table.resident.record_stream(torch.cuda.current_stream(dev))
+  return (resident, torch.empty((), dtype=torch.float32, device=dev),
+          torch.empty(table.workspace, dtype=torch.float64, device=dev))
+
+
 def clip_list_norm(table) -> torch.Tensor:
-  """Global norm of a `fused.TensorTable`.  The workspace is the call's own: tables are shared between streams."""
+  """Global norm of a `fused.TensorTable`."""
   index = table.device.index
   if _elsewhere(index):
     with torch.cuda.device(index):
       return clip_list_norm(table)
-  norm = torch.empty((), dtype=torch.float32, device=table.device)
-  ws = torch.empty(table.workspace, dtype=torch.float64, device=table.device)
-  table.list.global_norm(ws.data_ptr(), norm.data_ptr(), _current_stream(index))
+  stream = _current_stream(index)
+  resident, norm, ws = _clip_list_launch(table, stream)
+  table.list.global_norm(resident, ws.data_ptr(), norm.data_ptr(), stream)
   return norm
 
 
@@ -120,12 +149,12 @@ def clip_list_scale(table, clip_norm: float, use_norm: Optional[torch.Tensor]) -
   if _elsewhere(index):
     with torch.cuda.device(index):
       return clip_list_scale(table, clip_norm, use_norm)
+  stream = _current_stream(index)
+  resident, norm, ws = _clip_list_launch(table, stream)
   if use_norm is not None:
-    table.list.clip(0, use_norm.data_ptr(), clip_norm, 0, _current_stream(index))
+    table.list.clip(resident, 0, use_norm.data_ptr(), clip_norm, 0, stream)
     return use_norm
-  norm = torch.empty((), dtype=torch.float32, device=table.device)
-  ws = torch.empty(table.workspace, dtype=torch.float64, device=table.device)
-  table.list.clip(ws.data_ptr(), 0, clip_norm, norm.data_ptr(), _current_stream(index))
+  table.list.clip(resident, ws.data_ptr(), 0, clip_norm, norm.data_ptr(), stream)
   return norm
 
 
