@@ -24,12 +24,15 @@ ARCH = "gfx950"
 # of hipcc warns that it does not know the feature.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOURCES = ["conv_igemm.hip", "conv_pipe.hip", "conv_halo.hip", "conv_rows.hip", "conv_wgrad_rows.hip", "conv_wgrad.hip", "bn.hip", "pool.hip", "loss.hip", "optim.hip", "dense.hip", "residual_norm.hip",
+           "residual_norm_bf16.hip", "residual_norm_f16.hip", "residual_norm_f32.hip",
            "grad_clip.hip",
            "rccl_comm.cpp", "bindings.cpp"]
 HEADERS = ["common.h", "conv_params.h", "conv_epilogue.h", "elementwise.h", "rccl_comm.h"]
 # headers of one kernel file and the bindings
-OWN_HEADERS = {"residual_norm.hip": ["residual_norm.h"], "grad_clip.hip": ["grad_clip.h"],
-               "bindings.cpp": ["residual_norm.h", "grad_clip.h"]}
+_RESIDUAL_NORM = ["residual_norm.h", "residual_norm_kernels.h"]
+OWN_HEADERS = {"residual_norm.hip": _RESIDUAL_NORM, "residual_norm_bf16.hip": _RESIDUAL_NORM,
+               "residual_norm_f16.hip": _RESIDUAL_NORM, "residual_norm_f32.hip": _RESIDUAL_NORM,
+               "grad_clip.hip": ["grad_clip.h"], "bindings.cpp": ["residual_norm.h", "grad_clip.h"]}
 
 
 def so_path() -> str:

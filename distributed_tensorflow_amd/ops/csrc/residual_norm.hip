@@ -1,763 +1,18 @@
-// The seam between two residual blocks, forward and backward.
-//
-//   n = N(y) * post_gamma + post_beta          (n = y without post_gamma)
-//   h = x + scale * a(gate) * n                (a: identity or sigmoid; h = x without y)
-//   z = N(h) * pre_gamma + pre_beta            (the next block's input; none without pre_gamma)
-//
-// N normalises a row over its C channels: v / sqrt(mean v^2 + eps), or with `layer` (v - mean) / sqrt(var + eps).
-// Rows are pixels of an NHWC activation or tokens.  The work is a handful of operations per element, so memory
-// bounds it: every tensor is read once and written once, a row stays in registers (fp32) between its two
-// normalisations, and nothing but results goes back to memory.  z is taken from the unrounded h.
-//
-// Split: a lane owns eight consecutive channels (16 bytes of a 16-bit row).  Rows of up to 512 channels share a
-// wave (2 .. 64 lanes a row, sums by butterfly); wider rows take as many waves as they need, up to eight with one
-// or two chunks of eight channels a lane, and join their sums through LDS.
-//
-// Loads take any alignment (rows of odd length start anywhere); the last, partial chunk of a row goes element by element.
+// Entry points of the seam between two residual blocks: checks and the choice of the element type
+// (kernels: residual_norm_kernels.h).
 #include <algorithm>
 #include <stdexcept>
 
-#include "residual_norm.h"
+#include "residual_norm_kernels.h"
+
+extern template void rn::launch_fwd<DT_BF16>(const ResidualNormParams& p, hipStream_t s);
+extern template void rn::launch_fwd<DT_F16>(const ResidualNormParams& p, hipStream_t s);
+extern template void rn::launch_fwd<DT_F32>(const ResidualNormParams& p, hipStream_t s);
+extern template void rn::launch_bwd<DT_BF16>(const ResidualNormParams& p, hipStream_t s);
+extern template void rn::launch_bwd<DT_F16>(const ResidualNormParams& p, hipStream_t s);
+extern template void rn::launch_bwd<DT_F32>(const ResidualNormParams& p, hipStream_t s);
 
 namespace {
-
-// 16 bytes at the alignment of their elements: the memory system takes any address, one load all the same
-typedef u32x4 __attribute__((aligned(2))) Any16;
-typedef f32x4 __attribute__((aligned(4))) Any16F;
-
-// NT: past the caches (a sweep over more than they hold)
-template <bool NT, typename V>
-__device__ __forceinline__ V get16(const V* p) {
-  if constexpr (NT) return __builtin_nontemporal_load(p);
-  else return *p;
-}
-template <bool NT, typename V, typename W>
-__device__ __forceinline__ void put16(V* p, const W v) {
-  if constexpr (NT) __builtin_nontemporal_store((V)v, p);
-  else *p = v;
-}
-
-// Eight channels from `c` on of the row at `p`, as they sit in memory; what lies past channel C - 1 is zero.
-template <int DT, bool NT = false>
-__device__ __forceinline__ Raw8<DT> load_raw(const typename Elem<DT>::T* p, int c, int C) {
-  Raw8<DT> r = zero_raw<DT>();
-  if (c + 8 <= C) {
-    if constexpr (DT == DT_F32) {
-      r.lo = get16<NT>(reinterpret_cast<const Any16F*>(p + c));
-      r.hi = get16<NT>(reinterpret_cast<const Any16F*>(p + c + 4));
-    } else {
-      r.v = get16<NT>(reinterpret_cast<const Any16*>(p + c));
-    }
-  } else if (c < C) {
-    if constexpr (DT == DT_F32) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (c + j < C) r.lo[j] = p[c + j];
-        if (c + 4 + j < C) r.hi[j] = p[c + 4 + j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < C) r.v[j >> 1] |= (uint32_t)p[c + j] << (16 * (j & 1));
-    }
-  }
-  return r;
-}
-
-template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, int c, int C, float* f) {
-  unpack8<DT>(load_raw<DT>(p, c, C), f);
-}
-
-template <int DT, bool NT = false>
-__device__ __forceinline__ void store8(typename Elem<DT>::T* p, int c, int C, const float* f) {
-  if (c + 8 <= C) {
-    if constexpr (DT == DT_F32) {
-      put16<NT>(reinterpret_cast<Any16F*>(p + c), f32x4{f[0], f[1], f[2], f[3]});
-      put16<NT>(reinterpret_cast<Any16F*>(p + c + 4), f32x4{f[4], f[5], f[6], f[7]});
-    } else {
-      u32x4 v;
-      v.x = pack2<DT>(f[0], f[1]); v.y = pack2<DT>(f[2], f[3]);
-      v.z = pack2<DT>(f[4], f[5]); v.w = pack2<DT>(f[6], f[7]);
-      put16<NT>(reinterpret_cast<Any16*>(p + c), v);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < C) p[c + j] = from_f<DT>(f[j]);
-  }
-}
-
-// Rows of the results; `nt` is the same for a whole launch.
-template <int DT>
-__device__ __forceinline__ void store_row(void* to, int64_t at, int c, int C, const float* f, int nt) {
-  typename Elem<DT>::T* p = reinterpret_cast<typename Elem<DT>::T*>(to) + at;
-  if (nt) store8<DT, true>(p, c, C, f);
-  else store8<DT, false>(p, c, C, f);
-}
-
-// fp32 rows take the library's exponential and a true division, 16-bit rows the hardware's (their error, a few
-// 2^-22, vanishes in the rounding of the result).
-template <int DT>
-__device__ __forceinline__ float sigmoid_f(float g) {
-  if constexpr (DT == DT_F32) return 1.f / (1.f + expf(-g));
-  else return __builtin_amdgcn_rcpf(1.f + __expf(-g));
-}
-
-// v + v of the lane that is `O` away, in every lane (O = 1, 2, 4 .. 32 in this order: from O = 4 on the lanes of the
-// smaller groups hold the same value already, so a mirrored row does for an exchange).  Register to register: no trip
-// through LDS.
-template <int O>
-__device__ __forceinline__ float add_lane(float v) {
-  const int i = __float_as_int(v);
-  if constexpr (O == 1) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0xB1, 0xf, 0xf, true));
-  else if constexpr (O == 2) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x4E, 0xf, 0xf, true));
-  else if constexpr (O == 4) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x141, 0xf, 0xf, true));
-  else if constexpr (O == 8) return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x140, 0xf, 0xf, true));
-  else if constexpr (O == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
-    return __int_as_float(r[0]) + __int_as_float(r[1]);
-  } else {
-    const auto r = __builtin_amdgcn_permlane32_swap(i, i, false, false);
-    return __int_as_float(r[0]) + __int_as_float(r[1]);
-  }
-}
-
-// Sums of N values over the lanes of a row, given to all of them.  LPR lanes of a wave hold a narrow row; a wide one
-// has `waves` whole waves, joined through the half `turn & 1` of `red`: the barrier of the next sum separates this
-// sum's reads from the writes after next.
-template <int LPR, bool WIDE, int N>
-__device__ __forceinline__ void row_sums(float* v, float (*red)[4][8], int waves, int& turn) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = add_lane<1>(v[i]);
-    if constexpr (LPR >= 4) v[i] = add_lane<2>(v[i]);
-    if constexpr (LPR >= 8) v[i] = add_lane<4>(v[i]);
-    if constexpr (LPR >= 16) v[i] = add_lane<8>(v[i]);
-    if constexpr (LPR >= 32) v[i] = add_lane<16>(v[i]);
-    if constexpr (LPR >= 64) v[i] = add_lane<32>(v[i]);
-  }
-  if constexpr (WIDE) {
-    float (*mine)[8] = red[turn & 1];
-    ++turn;
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) mine[i][threadIdx.x >> 6] = v[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float s = 0.f;
-      for (int w = 0; w < waves; ++w) s += mine[i][w];
-      v[i] = s;
-    }
-  }
-}
-
-// Subtracts the mean of the row from its channels (and leaves those past the end zero).
-template <int K>
-__device__ __forceinline__ void centre(float (*v)[8], const int* c, int C, float mean) {
-  if (C % 8 == 0) {       // a lane's channels are all there or none is
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const float m = c[k] < C ? mean : 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] -= m;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] = c[k] + j < C ? v[k][j] - mean : 0.f;
-  }
-}
-
-// Centres `v` (LAYER) and returns 1 / sqrt(mean square + eps) of the row.
-template <int LPR, bool WIDE, int K, bool LAYER>
-__device__ __forceinline__ float normalise(float (*v)[8], const int* c, int C, float inv_c, float eps,
-                                           float (*red)[4][8], int waves, int& turn) {
-  float s[1];
-  if constexpr (LAYER) {
-    s[0] = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[0] += v[k][j];
-    row_sums<LPR, WIDE, 1>(s, red, waves, turn);
-    centre<K>(v, c, C, s[0] * inv_c);
-  }
-  s[0] = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[0] += v[k][j] * v[k][j];
-  row_sums<LPR, WIDE, 1>(s, red, waves, turn);
-  return 1.f / sqrtf(s[0] * inv_c + eps);
-}
-
-template <int DT, int K>
-struct FwdIn {
-  Raw8<DT> x[K], y[K], gate[K];
-  Raw8<DT_F32> group[K];
-};
-
-template <int DT, int K, bool NT>
-__device__ __forceinline__ void load_fwd(FwdIn<DT, K>& in, const ResidualNormParams& p, int64_t r, const int* c, int C) {
-  typedef typename Elem<DT>::T T;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    in.x[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], C);
-    if (p.y) in.y[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
-    if (p.gate_mode == GATE_ELEMENT)
-      in.gate[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
-    if (p.gate_mode == GATE_GROUP)
-      in.group[k] = load_raw<DT_F32>(reinterpret_cast<const float*>(p.gate) +
-                                         (int64_t)((uint32_t)r / (uint32_t)p.group_rows) * p.ldgate, c[k], C);
-  }
-}
-
-// The blocks walk the rows side by side: while one row's sums are taken the next one's loads are under way, and the
-// vectors stay in registers.
-// Waves per SIMD that the registers are kept small enough for.
-constexpr int fwd_waves(int dt, bool layer, int chunks) { return chunks > 1 ? 2 : layer && dt == DT_F32 ? 3 : 4; }
-
-template <int DT, int LPR, bool WIDE, int K, bool LAYER>
-__global__ __launch_bounds__(WIDE ? 512 : 256, fwd_waves(DT, LAYER, K)) void fwd_kernel(const ResidualNormParams p,
-                                                                                              const int nt) {
-  __shared__ float red[2][4][8];
-  int turn = 0;
-  const int lanes = WIDE ? (int)blockDim.x : LPR;
-  const int waves = WIDE ? (int)(blockDim.x >> 6) : 1;
-  const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x % LPR);
-  const int slots = WIDE ? 1 : 256 / LPR;
-  const int slot = WIDE ? 0 : (int)(threadIdx.x / LPR);
-  const int C = p.C;
-  const float inv_c = 1.f / (float)C;
-  int c[K];
-  float pw[K][8], pb[K][8], qw[K][8], qb[K][8], g[K][8];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    c[k] = (lane + k * lanes) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { pw[k][j] = pb[k][j] = qw[k][j] = qb[k][j] = 0.f; g[k][j] = 1.f; }
-    if (p.post_gamma) load8<DT_F32>(p.post_gamma, c[k], C, pw[k]);
-    if (LAYER && p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, pb[k]);
-    if (p.pre_gamma) load8<DT_F32>(p.pre_gamma, c[k], C, qw[k]);
-    if (LAYER && p.pre_beta) load8<DT_F32>(p.pre_beta, c[k], C, qb[k]);
-  }
-  // every lane of a wave walks the same number of passes (the sums need all of them); a row past the run's end has
-  // no channels: zeros are read and nothing is written for it
-  const int64_t row0 = (int64_t)blockIdx.x * slots, row1 = p.P, step = (int64_t)gridDim.x * slots;
-  FwdIn<DT, K> next;
-  auto ask = [&](int64_t base) {
-    if (base >= row1) return;
-    const int Cr = base + slot < row1 ? C : 0;
-    const int64_t r = base + slot < row1 ? base + slot : 0;
-    if (nt) load_fwd<DT, K, true>(next, p, r, c, Cr);
-    else load_fwd<DT, K, false>(next, p, r, c, Cr);
-  };
-  ask(row0);
-  for (int64_t base = row0; base < row1; base += step) {
-    const FwdIn<DT, K> in = next;
-    const int64_t r = base + slot < row1 ? base + slot : 0;
-    const int Cr = base + slot < row1 ? C : 0;
-    ask(base + step);
-    float h[K][8], v[K][8];
-#pragma unroll
-    for (int k = 0; k < K; ++k) unpack8<DT>(in.x[k], h[k]);
-    if (p.y) {
-      if (p.gate_mode != GATE_NONE) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (p.gate_mode == GATE_GROUP) unpack8<DT_F32>(in.group[k], g[k]);
-          else unpack8<DT>(in.gate[k], g[k]);
-          if (p.sigmoid) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) unpack8<DT>(in.y[k], v[k]);
-      if (p.post_gamma) {
-        const float rs = normalise<LPR, WIDE, K, LAYER>(v, c, Cr, inv_c, p.eps, red, waves, turn);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] = LAYER ? v[k][j] * rs * pw[k][j] + pb[k][j] : v[k][j] * rs * pw[k][j];
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[k][j] += p.scale * (g[k][j] * v[k][j]);
-        store_row<DT>(p.h, r * C, c[k], Cr, h[k], nt);
-      }
-    }
-    if (p.pre_gamma) {
-      const float rs = normalise<LPR, WIDE, K, LAYER>(h, c, Cr, inv_c, p.eps, red, waves, turn);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[k][j] = LAYER ? h[k][j] * rs * qw[k][j] + qb[k][j] : h[k][j] * rs * qw[k][j];
-        store_row<DT>(p.z, r * C, c[k], Cr, h[k], nt);
-      }
-    }
-  }
-}
-
-// ---- backward ----------------------------------------------------------------------------------
-//   H  = dh + r_h (dz' - [mean dz'] - hat_h mean(dz' hat_h))        dz' = dz * pre_gamma,  hat_h = N(h)
-//   dx = H        up = scale * H        dgate = up * n * a'(gate)   dn = up * a(gate)
-//   dy = r_y (t - [mean t] - hat_y mean(t hat_y))                   t = dn * post_gamma,   hat_y = N(y)
-//   dpre_gamma = sum dz hat_h   dpre_beta = sum dz   dpost_gamma = sum dn hat_y   dpost_beta = sum dn
-// (the bracketed means only with `layer`).  The statistics are taken again from h and y, which are in registers
-// anyway: two sums more per row instead of saved tensors that could belong to another call.
-// A lane keeps its channels for all of its block's rows, so the sums over rows are registers; blocks leave one row of
-// partial sums each and finish_kernel adds them in a fixed order (no atomics: the same bits every time).
-//
-// A block's rows lie in one group (of rows that share a gate row), or it owns whole groups; where a group has fewer
-// rows than the block has row slots, every slot owns whole groups of its own (`own_groups`).
-
-struct BwdPlan {
-  int blocks;        // grid
-  int parts;         // blocks per group
-  int groups;        // groups of rows (1 without a group gate)
-  int group_rows;
-  int own_groups;    // each row slot takes whole groups
-  int nt;            // more bytes than the memory-side cache holds: loads and stores past the caches
-};
-
-// Waves per SIMD that the backward kernel is built for: its registers (sums over rows, weights, a row in work and the
-// next one's loads) leave room for two, three for RMS norms of 16-bit rows.  The grid is what is resident at once:
-// one round of blocks, no half-empty second one.
-constexpr int bwd_waves(int dt, bool layer, int chunks) { return !layer && dt != DT_F32 && chunks == 1 ? 3 : 2; }
-
-int narrow_lanes(int C) {       // lanes a row of up to 512 channels
-  int l = 2;
-  while (l * 8 < C) l *= 2;
-  return l;
-}
-
-int wide_threads(int C) {
-  const int per_wave = C <= 4096 ? 512 : 1024;
-  return 64 * ((C + per_wave - 1) / per_wave);
-}
-
-// Whether `tensors` tensors of the rows are more than the 256 MB that the memory-side cache holds.
-int big(const ResidualNormParams& p, int tensors) {
-  return (int64_t)p.P * p.C * (p.dt == DT_F32 ? 4 : 2) * tensors > (256ll << 20);
-}
-
-// Sweeps over more than the cache holds run best as a narrow front: eight waves a CU and accesses past the caches
-// (200704 x 512 bf16 with a gate per image: 140 us; 158 with sixteen waves, 206 through the caches; the gradient with
-// a gate per element: 286; 312 with twelve).  What the cache holds wants every wave there is room for (4099 x 1001
-// fp16: 48, 27, 18, 14, 13 us with 2, 4, 8, 16, 32 waves a CU).
-int fwd_blocks(const ResidualNormParams& p, int nt) {
-  const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
-  const int waves = (p.C <= 512 ? 256 : wide_threads(p.C)) / 64;
-  const int most = 256 * std::max(1, (nt ? 8 : 32) / waves);
-  const int64_t want = ((int64_t)p.P + slots - 1) / slots;
-  return (int)(want < most ? want : most);
-}
-
-BwdPlan plan_bwd(const ResidualNormParams& p) {
-  BwdPlan b;
-  const bool grouped = p.gate_mode == GATE_GROUP;
-  b.group_rows = grouped ? p.group_rows : p.P;
-  b.groups = p.P / b.group_rows;
-  const int slots = p.C <= 512 ? 256 / narrow_lanes(p.C) : 1;
-  const int waves = (p.C <= 512 ? 256 : wide_threads(p.C)) / 64;
-  b.nt = big(p, 6);
-  // the grid is what is resident at once: no half-empty second round of blocks
-  const int resident = 256 * std::max(1, 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2) / waves);
-  const int want = b.nt && !grouped ? std::min(resident, 256 * std::max(1, 8 / waves)) : resident;
-  b.own_groups = grouped && slots > 1 && b.group_rows < 4 * slots;
-  if (b.own_groups) {
-    const int sets = (b.groups + slots - 1) / slots;
-    b.blocks = sets < want ? sets : want;
-    b.parts = 1;
-    return b;
-  }
-  b.parts = 1;
-  if (b.groups == 1) {
-    b.parts = std::min((b.group_rows + slots - 1) / slots, want);      // a part has work for every slot
-    b.blocks = b.parts;
-  } else if (b.groups < 4 * want) {
-    // as many parts as leave the fewest rows to the busiest slot on the grid (a few percent are worth fewer partial sums)
-    const int most = std::min((b.group_rows + slots - 1) / slots, std::max(16, want / b.groups));
-    double best = 1e30;
-    for (int parts = 1; parts <= most; ++parts) {
-      const int64_t rounds = ((int64_t)b.groups * parts + want - 1) / want;
-      if (rounds > 1 && parts > 16) break;
-      const double rows = (double)rounds * ((b.group_rows + (int64_t)parts * slots - 1) / ((int64_t)parts * slots));
-      if (rows * (rounds > 1 ? 1.05 : 1.0) < 0.97 * best) { best = rows * (rounds > 1 ? 1.05 : 1.0); b.parts = parts; }
-    }
-    b.blocks = b.groups * b.parts;
-  } else {
-    b.blocks = want;
-  }
-  return b;
-}
-
-// Partial sums: [vector][block][C]; which vectors are kept goes by the gradients asked for.
-struct Partials {
-  float* row[5];      // dpre_gamma, dpost_gamma, dpre_beta, dpost_beta, dgate
-};
-
-// The tensors of a row as they sit in memory.
-template <int DT, int K>
-struct RowIn {
-  Raw8<DT> dh[K], dz[K], h[K], y[K], gate[K];
-};
-
-template <int DT, int K, bool NT>
-__device__ __forceinline__ void load_row(RowIn<DT, K>& in, const ResidualNormParams& p, int64_t r, const int* c, int C) {
-  typedef typename Elem<DT>::T T;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    in.dh[k] = zero_raw<DT>();
-    if (p.dh) in.dh[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.dh) + r * p.lddh, c[k], C);
-    if (p.dz) {
-      in.dz[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.dz) + r * p.lddz, c[k], C);
-      in.h[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.x) + r * p.ldx, c[k], C);
-    }
-    if (p.y) in.y[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.y) + r * p.ldy, c[k], C);
-    if (p.gate_mode == GATE_ELEMENT)
-      in.gate[k] = load_raw<DT, NT>(reinterpret_cast<const T*>(p.gate) + r * p.ldgate, c[k], C);
-  }
-}
-
-template <int DT, int LPR, bool WIDE, int K, bool LAYER, bool GROUP>
-__global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
-                                                               const Partials part) {
-  typedef typename Elem<DT>::T T;
-  // sums over rows: of the two gammas, with LAYER of the two betas, with GROUP of the gate
-  constexpr int SUMS = 2 + (LAYER ? 2 : 0) + (GROUP ? 1 : 0), GATE = SUMS - 1;
-  __shared__ float red[2][4][8];
-  __shared__ float join[WIDE ? 1 : 256 * 8];
-  int turn = 0;
-  const int nt = plan.nt;
-  const int lanes = WIDE ? (int)blockDim.x : LPR;
-  const int waves = WIDE ? (int)(blockDim.x >> 6) : 1;
-  const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x % LPR);
-  const int slots = WIDE ? 1 : 256 / LPR;
-  const int slot = WIDE ? 0 : (int)(threadIdx.x / LPR);
-  const int C = p.C;
-  const float inv_c = 1.f / (float)C;
-  int c[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) c[k] = (lane + k * lanes) * 8;
-  float acc[SUMS][K][8];
-#pragma unroll
-  for (int i = 0; i < SUMS; ++i)
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][k][j] = 0.f;
-  float pw[K][8], pb[K][8], qw[K][8];     // post_gamma, post_beta, pre_gamma
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { pw[k][j] = 1.f; pb[k][j] = qw[k][j] = 0.f; }
-    if (p.post_gamma) load8<DT_F32>(p.post_gamma, c[k], C, pw[k]);
-    if (LAYER && p.post_beta) load8<DT_F32>(p.post_beta, c[k], C, pb[k]);
-    if (p.pre_gamma) load8<DT_F32>(p.pre_gamma, c[k], C, qw[k]);
-  }
-  // the sets of groups this block works on, and the rows of a group that are its own
-  const int per_set = plan.own_groups ? slots : 1;
-  const int first_set = plan.parts > 1 ? (int)blockIdx.x / plan.parts : (int)blockIdx.x;
-  const int stride_set = plan.parts > 1 ? plan.groups : (int)gridDim.x;      // parts > 1: one group a block
-  const int sets = (plan.groups + per_set - 1) / per_set;
-  const int row0 = plan.parts > 1 ? ((int)blockIdx.x % plan.parts) * slots : 0;
-  const int row1 = plan.group_rows;
-  const int step = plan.own_groups ? 1 : slots * plan.parts;     // the blocks of a group walk its rows side by side
-  for (int set = first_set; set < sets; set += stride_set) {
-    const int group = plan.own_groups ? set * slots + slot : set;
-    const bool group_live = group < plan.groups;
-    float g[K][8];
-    if constexpr (GROUP) {
-      const float* row_g = reinterpret_cast<const float*>(p.gate) + (int64_t)(group_live ? group : 0) * p.ldgate;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        load8<DT_F32>(row_g, c[k], C, g[k]);
-        if (p.sigmoid) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
-        }
-      }
-    }
-    // a row that is not there has no channels: zeros are read and nothing is written for it
-    auto row_of = [&](int rr, int64_t* r) {
-      const int in_group = plan.own_groups ? rr : rr + slot;
-      const bool live = group_live && in_group < row1;
-      *r = live ? (int64_t)group * plan.group_rows + in_group : 0;
-      return live ? C : 0;
-    };
-    // the next row's loads are under way while this row's sums are taken
-    RowIn<DT, K> next;
-    auto ask = [&](int rr) {
-      if (rr >= row1) return;
-      int64_t r;
-      const int Cr = row_of(rr, &r);
-      if (nt) load_row<DT, K, true>(next, p, r, c, Cr);
-      else load_row<DT, K, false>(next, p, r, c, Cr);
-    };
-    ask(row0);
-    for (int rr = row0; rr < row1; rr += step) {
-      const RowIn<DT, K> in = next;
-      int64_t r;
-      const int Cr = row_of(rr, &r);
-      ask(rr + step);
-      float up[K][8], h[K][8], v[K][8];
-#pragma unroll
-      for (int k = 0; k < K; ++k) unpack8<DT>(in.dh[k], up[k]);
-      float s[3] = {0.f, 0.f, 0.f};
-      float rs = 1.f, m_d = 0.f;
-      if (p.y) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) unpack8<DT>(in.y[k], v[k]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
-      }
-      if (p.dz) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) unpack8<DT>(in.h[k], h[k]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) h[k][j] = 0.f;
-      }
-      if (p.dz || p.post_gamma) {
-        // both norms' statistics and what the first gradient needs come from the same sums
-        if constexpr (LAYER) {
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            float dz[8];
-            if (p.dz) unpack8<DT>(in.dz[k], dz);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              s[0] += h[k][j];
-              s[1] += v[k][j];
-              if (p.dz) s[2] += dz[j] * qw[k][j];
-            }
-          }
-          row_sums<LPR, WIDE, 3>(s, red, waves, turn);
-          const float mean_h = s[0] * inv_c, mean_y = p.post_gamma ? s[1] * inv_c : 0.f;
-          m_d = s[2] * inv_c;
-          centre<K>(h, c, Cr, mean_h);
-          centre<K>(v, c, Cr, mean_y);
-          s[0] = s[1] = s[2] = 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          float dz[8];
-          if (p.dz) unpack8<DT>(in.dz[k], dz);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            s[0] += h[k][j] * h[k][j];
-            s[1] += v[k][j] * v[k][j];
-            if (p.dz) s[2] += dz[j] * qw[k][j] * h[k][j];
-          }
-        }
-        row_sums<LPR, WIDE, 3>(s, red, waves, turn);
-        if (p.post_gamma) rs = 1.f / sqrtf(s[1] * inv_c + p.eps);
-      }
-      if (p.dz) {
-        const float rh = 1.f / sqrtf(s[0] * inv_c + p.eps), m_dot = s[2] * rh * inv_c;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          float dz[8];
-          unpack8<DT>(in.dz[k], dz);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float hat = h[k][j] * rh;
-            const float d = LAYER ? dz[j] * qw[k][j] - m_d : dz[j] * qw[k][j];
-            up[k][j] += rh * (d - hat * m_dot);
-            acc[0][k][j] += dz[j] * hat;
-            if constexpr (LAYER) acc[2][k][j] += dz[j];
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) store_row<DT>(p.dx, r * C, c[k], Cr, up[k], nt);
-      if (!p.y) continue;
-      float t[2] = {0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float a[8], dg[8];
-        if constexpr (!GROUP) {
-          if (p.gate_mode == GATE_ELEMENT) unpack8<DT>(in.gate[k], a);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          // (channels past the end: gamma is zero, so they add nothing to the row's sums; their own are not stored)
-          const float u = p.scale * up[k][j];
-          const float hat = v[k][j] * rs;
-          const float n = LAYER ? hat * pw[k][j] + pb[k][j] : hat * pw[k][j];
-          float dn = u;
-          dg[j] = u * n;
-          if constexpr (GROUP) {
-            dn *= g[k][j];
-            acc[GATE][k][j] += dg[j];
-          } else if (p.gate_mode == GATE_ELEMENT) {
-            if (p.sigmoid) {
-              a[j] = sigmoid_f<DT>(a[j]);
-              dg[j] *= a[j] * (1.f - a[j]);
-            }
-            dn *= a[j];
-          }
-          acc[1][k][j] += dn * hat;
-          if constexpr (LAYER) acc[3][k][j] += dn;
-          v[k][j] = hat;
-          up[k][j] = dn * pw[k][j];
-          t[0] += up[k][j] * hat;
-          t[1] += up[k][j];
-        }
-        if constexpr (!GROUP) {
-          if (p.gate_mode == GATE_ELEMENT) store_row<DT>(p.dgate, r * C, c[k], Cr, dg, nt);
-        }
-      }
-      if (p.post_gamma) {
-        row_sums<LPR, WIDE, LAYER ? 2 : 1>(t, red, waves, turn);
-        const float m_dot = t[0] * inv_c, m_t = LAYER ? t[1] * inv_c : 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) up[k][j] = rs * (up[k][j] - m_t - v[k][j] * m_dot);
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) store_row<DT>(p.dy, r * C, c[k], Cr, up[k], nt);
-    }
-    if (GROUP && plan.parts == 1) {
-      // whole groups: the gate's gradient is complete here
-      if constexpr (!WIDE) {
-        if (!plan.own_groups) {       // summed over the slots, lane by lane of slot 0
-          __syncthreads();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) join[slot * LPR * 8 + lane * 8 + j] = acc[GATE][0][j];
-          __syncthreads();
-          if (slot == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {       // eight sums of `slots` values each, once a group
-              float sum = 0.f;
-#pragma unroll 4
-              for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + lane * 8 + j];
-              acc[GATE][0][j] = sum;
-            }
-          }
-        }
-      }
-      if (group_live && (WIDE || plan.own_groups || slot == 0)) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (p.sigmoid) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[GATE][k][j] *= g[k][j] * (1.f - g[k][j]);
-          }
-          store8<DT_F32>(reinterpret_cast<float*>(p.dgate) + (int64_t)group * C, c[k], C, acc[GATE][k]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[GATE][k][j] = 0.f;
-    }
-  }
-  // the block's row of partial sums
-#pragma unroll
-  for (int i = 0; i < SUMS; ++i) {
-    float* to = part.row[GROUP && i == GATE ? 4 : i];
-    if (!to) continue;
-    to += (int64_t)blockIdx.x * C;
-    if constexpr (WIDE) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) store8<DT_F32>(to, c[k], C, acc[i][k]);
-    } else {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) join[slot * LPR * 8 + lane * 8 + j] = acc[i][0][j];
-      __syncthreads();
-      for (int col = threadIdx.x; col < C; col += 256) {
-        float sum = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < slots; ++q) sum += join[q * LPR * 8 + col];
-        to[col] = sum;
-      }
-    }
-  }
-}
-
-// Sums the blocks' partial rows, in one launch.  The vectors' rows (all blocks') and a gate's (of one group, `parts`
-// of them) are taken 32 columns a block in 32 slices; gates of few parts go a column a thread, 1024 a block, where
-// slices would leave most of a block idle (256 groups of 4 parts, 2048 columns: 35 us in slices, 5 us this way).
-struct Finish {
-  const float* from[5];
-  float* to[5];
-  const float* gate;
-  int64_t ldgate;
-  int C, rows, parts, groups, sigmoid;
-  int vector_blocks;      // blocks of the vectors; the gate's follow
-};
-constexpr int FEW_PARTS = 32;
-
-template <int DT>
-__global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
-  __shared__ float join[32][33];
-  const int cols = (f.C + 31) / 32;
-  int b = (int)blockIdx.x, i = 4, group = 0, rows = f.parts, col;
-  if (b < f.vector_blocks) {
-    // the b / cols-th vector that is wanted
-    int skip = b / cols;
-    i = 0;
-    while (f.to[i] == nullptr || skip-- > 0) ++i;
-    b %= cols;
-    rows = f.rows;
-  } else {
-    b -= f.vector_blocks;
-    if (f.parts <= FEW_PARTS) {
-      const int wide_cols = (f.C + 1023) / 1024;
-      group = b / wide_cols;
-      col = (b % wide_cols) * 1024 + (int)threadIdx.x;
-      if (col >= f.C) return;
-      const float* from = f.from[4] + (int64_t)group * f.parts * f.C + col;
-      float sum = 0.f;
-#pragma unroll 4
-      for (int r = 0; r < f.parts; ++r) sum += from[(int64_t)r * f.C];
-      if (f.sigmoid) {
-        const float sg = sigmoid_f<DT>(f.gate[(int64_t)group * f.ldgate + col]);
-        sum *= sg * (1.f - sg);
-      }
-      f.to[4][(int64_t)group * f.C + col] = sum;
-      return;
-    }
-    group = b / cols;
-    b %= cols;
-  }
-  col = b * 32 + (threadIdx.x & 31);
-  const int slice = threadIdx.x >> 5;
-  float sum = 0.f;
-  if (col < f.C) {
-    const float* from = f.from[i] + (int64_t)group * f.parts * f.C + col;
-#pragma unroll 16
-    for (int r = slice; r < rows; r += 32) sum += from[(int64_t)r * f.C];
-  }
-  join[slice][threadIdx.x & 31] = sum;
-  __syncthreads();
-  if (slice == 0 && col < f.C) {
-    sum = 0.f;
-#pragma unroll
-    for (int q = 0; q < 32; ++q) sum += join[q][threadIdx.x];
-    if (i == 4 && f.sigmoid) {
-      const float sg = sigmoid_f<DT>(f.gate[(int64_t)group * f.ldgate + col]);
-      sum *= sg * (1.f - sg);
-    }
-    f.to[i][(int64_t)group * f.C + col] = sum;
-  }
-}
 
 void check(const ResidualNormParams& p) {
   if (p.C < 1 || p.C > RESIDUAL_NORM_MAX_C) throw std::invalid_argument("residual_norm: 1 to 8192 channels");
@@ -771,38 +26,18 @@ void check(const ResidualNormParams& p) {
     throw std::invalid_argument("residual_norm: a beta goes with its gamma and with norm='layer'");
 }
 
-// (lanes per row, wide, chunks per lane) by the row's length alone: eight channels a lane while that takes at most
-// 512 threads, sixteen above.
-#define DTF_ROW_SWITCH(C, ...)                                                                     \
-  do {                                                                                             \
-    if ((C) <= 16) { constexpr int LPR = 2, K = 1; constexpr bool WIDE = false; __VA_ARGS__; }      \
-    else if ((C) <= 32) { constexpr int LPR = 4, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
-    else if ((C) <= 64) { constexpr int LPR = 8, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
-    else if ((C) <= 128) { constexpr int LPR = 16, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
-    else if ((C) <= 256) { constexpr int LPR = 32, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
-    else if ((C) <= 512) { constexpr int LPR = 64, K = 1; constexpr bool WIDE = false; __VA_ARGS__; } \
-    else if ((C) <= 4096) { constexpr int LPR = 64, K = 1; constexpr bool WIDE = true; __VA_ARGS__; } \
-    else { constexpr int LPR = 64, K = 2; constexpr bool WIDE = true; __VA_ARGS__; }                \
-  } while (0)
-
-
 }  // namespace
 
 size_t residual_norm_workspace_floats(const ResidualNormParams& p) {
   if (p.P <= 0 || p.C < 1 || (p.gate_mode == GATE_GROUP && p.group_rows < 1)) return 0;
-  return (size_t)5 * plan_bwd(p).blocks * p.C;
+  // enough for either kind of kernel: the caller need not know which one its call takes
+  return (size_t)5 * std::max(rn::plan_bwd(p, true).blocks, rn::plan_bwd(p, false).blocks) * p.C;
 }
 
 void launch_residual_norm_fwd(const ResidualNormParams& p, hipStream_t s) {
   check(p);
   if (p.P == 0) return;
-  const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
-  const int nt = big(p, 4), blocks = fwd_blocks(p, nt);
-#define DTF_FWD(LAYER)                                                                                         \
-  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((fwd_kernel<DT, LPR, WIDE, K, LAYER>), dim3(blocks), \
-                                                             dim3(threads), 0, s, p, nt)))
-  if (p.layer) { DTF_FWD(true); } else { DTF_FWD(false); }
-#undef DTF_FWD
+  DTF_DT_SWITCH(p.dt, rn::launch_fwd<DT>(p, s));
 }
 
 void launch_residual_norm_bwd(const ResidualNormParams& p, hipStream_t s) {
@@ -811,37 +46,5 @@ void launch_residual_norm_bwd(const ResidualNormParams& p, hipStream_t s) {
   if ((p.dz != nullptr) != (p.pre_gamma != nullptr))
     throw std::invalid_argument("residual_norm_grad: dz goes with pre_gamma");
   if (!p.dz && !p.dh) throw std::invalid_argument("residual_norm_grad: neither dh nor dz");
-  const BwdPlan plan = plan_bwd(p);
-  const int threads = p.C <= 512 ? 256 : wide_threads(p.C);
-  float* to[5] = {p.dpre_gamma, p.dpost_gamma, p.dpre_beta, p.dpost_beta, nullptr};
-  if (p.gate_mode == GATE_GROUP && plan.parts > 1) to[4] = reinterpret_cast<float*>(p.dgate);
-  Partials part;
-  Finish f;
-  int vectors = 0;
-  for (int i = 0; i < 5; ++i) {
-    part.row[i] = to[i] ? p.ws + (size_t)i * plan.blocks * p.C : nullptr;
-    f.from[i] = part.row[i];
-    f.to[i] = to[i];
-    vectors += i < 4 && to[i];
-  }
-#define DTF_BWD(LAYER, GROUP)                                                                                  \
-  DTF_DT_SWITCH(p.dt, DTF_ROW_SWITCH(p.C, hipLaunchKernelGGL((bwd_kernel<DT, LPR, WIDE, K, LAYER, GROUP>),      \
-                                                             dim3(plan.blocks), dim3(threads), 0, s, p, plan, part)))
-  if (p.layer) {
-    if (p.gate_mode == GATE_GROUP) { DTF_BWD(true, true); } else { DTF_BWD(true, false); }
-  } else {
-    if (p.gate_mode == GATE_GROUP) { DTF_BWD(false, true); } else { DTF_BWD(false, false); }
-  }
-#undef DTF_BWD
-  if (!vectors && !to[4]) return;
-  f.gate = reinterpret_cast<const float*>(p.gate);
-  f.ldgate = p.ldgate;
-  f.C = p.C;
-  f.rows = plan.blocks;
-  f.parts = plan.parts;
-  f.groups = plan.groups;
-  f.sigmoid = p.sigmoid;
-  f.vector_blocks = vectors * ((p.C + 31) / 32);
-  const int gates = to[4] ? plan.groups * (plan.parts <= FEW_PARTS ? (p.C + 1023) / 1024 : (p.C + 31) / 32) : 0;
-  DTF_DT_SWITCH(p.dt, hipLaunchKernelGGL(finish_kernel<DT>, dim3(f.vector_blocks + gates), dim3(1024), 0, s, f));
+  DTF_DT_SWITCH(p.dt, rn::launch_bwd<DT>(p, s));
 }

@@ -48,9 +48,8 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _FP32 = torch.float32
 
 
-def _row_pitch(name: str, t: torch.Tensor) -> int:
+def _row_pitch(name: str, t: torch.Tensor, channels: int) -> int:
   """Elements from one row of `t` to the next; rows are everything but the last dimension."""
-  channels = t.shape[-1]
   if t.is_contiguous():
     return channels
   if channels > 1 and t.stride(-1) != 1:
@@ -67,11 +66,11 @@ def _row_pitch(name: str, t: torch.Tensor) -> int:
   return pitch
 
 
-def _pitch(name: str, t: torch.Tensor, shape, dtype, device: int) -> int:
+def _pitch(name: str, t: torch.Tensor, channels: int, shape, dtype, device: int) -> int:
   if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
     raise ValueError("%s: %s %s on %s, but the rows are %s %s on device %d" % (
         name, tuple(t.shape), t.dtype, t.device, tuple(shape), dtype, device))
-  return _row_pitch(name, t)
+  return _row_pitch(name, t, channels)
 
 
 def _seam(like, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, norm, eps):
@@ -107,13 +106,13 @@ def _seam(like, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta, n
   group_rows, gate_pitch = 0, c
   if gate is not None:
     if gate.dtype is dtype and gate.shape == shape:
-      gate_pitch = _pitch("gate", gate, shape, dtype, device)
+      gate_pitch = _pitch("gate", gate, c, shape, dtype, device)
     elif gate.dtype is _FP32 and gate.get_device() == device and gate.dim() in (1, 2) and gate.shape[-1] == c:
       groups = gate.numel() // c
       if groups < 1 or rows % groups:
         raise ValueError("gate: %d rows of it do not divide %d rows" % (groups, rows))
       group_rows = rows // groups
-      gate_pitch = _row_pitch("gate", gate)
+      gate_pitch = _row_pitch("gate", gate, c)
     else:
       raise ValueError("gate: one value per element in the rows' type, or float32 [groups, %d] with groups that "
                        "divide the rows; got %s %s on %s" % (c, tuple(gate.shape), gate.dtype, gate.device))
@@ -172,8 +171,8 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_gam
   rows, c, group_rows, ldgate, sigmoid, layer = _seam(x, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta,
                                                       norm, eps)
   _no_graph(x, y, post_gamma, post_beta, gate, pre_gamma, pre_beta)
-  ldx = _row_pitch("x", x)
-  ldy = c if y is None else _pitch("y", y, x.shape, x.dtype, x.get_device())
+  ldx = _row_pitch("x", x, c)
+  ldy = c if y is None else _pitch("y", y, c, x.shape, x.dtype, x.get_device())
   if x.is_cuda:
     if c > MAX_CHANNELS:
       raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, c))
@@ -217,10 +216,10 @@ def residual_norm_grad(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], h
   if dz is None and dh is None:
     raise ValueError("neither dh nor dz")
   shape, dtype, device = h.shape, h.dtype, h.get_device()
-  ldh = _row_pitch("h", h)
-  lddh = c if dh is None else _pitch("dh", dh, shape, dtype, device)
-  lddz = c if dz is None else _pitch("dz", dz, shape, dtype, device)
-  ldy = c if y is None else _pitch("y", y, shape, dtype, device)
+  ldh = _row_pitch("h", h, c)
+  lddh = c if dh is None else _pitch("dh", dh, c, shape, dtype, device)
+  lddz = c if dz is None else _pitch("dz", dz, c, shape, dtype, device)
+  ldy = c if y is None else _pitch("y", y, c, shape, dtype, device)
   if h.is_cuda:
     if c > MAX_CHANNELS:
       raise ValueError("at most %d channels, got %d" % (MAX_CHANNELS, c))
