@@ -325,8 +325,30 @@ void conv_pipe_kernel(const ConvParams p) {
       for (int mr = 0; mr < MR; ++mr)
         xf[mr] = *reinterpret_cast<const u32x4*>(st + (xoff[mr] ^ (ks << 6)));
       if constexpr (INBN) {
+        // eight-wave fp16 tiles sit at their 128 registers: the constants come in two halves, applied to every
+        // fragment before the next half is read (same arithmetic, no spill)
+        constexpr bool HALVES = NW == 8 && DT == DT_F16;
         // the lane's eight reduction channels of this step: kt * BK + ks * 32 + fq * 8 ...
         const float* tsc = bntab + kt * BK + ks * 32 + fq * 8;
+        if constexpr (HALVES) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const f32x4 sc = *reinterpret_cast<const f32x4*>(tsc + half * 4);
+            const f32x4 sh = *reinterpret_cast<const f32x4*>(tsc + INBN_KMAX + half * 4);
+#pragma unroll
+            for (int mr = 0; mr < MR; ++mr)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                xf[mr][half * 2 + j] = bn_relu_pair<DT>(xf[mr][half * 2 + j], sc[2 * j], sc[2 * j + 1], sh[2 * j], sh[2 * j + 1]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int mr = 0; mr < MR; ++mr)
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+              acc[nr][mr] = mfma_step<DT>(wf[nr], xf[mr], acc[nr][mr]);
+          continue;
+        }
         const f32x4 sa = *reinterpret_cast<const f32x4*>(tsc), sb = *reinterpret_cast<const f32x4*>(tsc + 4);
         const f32x4 ha = *reinterpret_cast<const f32x4*>(tsc + INBN_KMAX),
                     hb = *reinterpret_cast<const f32x4*>(tsc + INBN_KMAX + 4);
