@@ -291,6 +291,7 @@ class TensorTable:
     if len(self.out) != len(self.tensors):
       raise ValueError("%d outputs for %d tensors" % (len(self.out), len(self.tensors)))
     self.device = self.tensors[0].device
+    self.held = []          # every device table written so far: a captured graph may still read an older one
     self._build()
 
   def _build(self):
@@ -417,8 +418,8 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
     raise ValueError("clipped_sgd_momentum_l2: no parameters")
   if not clip_norm > 0:
     raise ValueError("clip_norm has to be positive, got %r" % clip_norm)
-  spans = [_span(params), _span(grads), _span(l2x2)] + ([_span(velocity)] if momentum else [])
-  if _overlaps(spans):
+  at = sorted([params.data_ptr(), grads.data_ptr(), l2x2.data_ptr()] + ([velocity.data_ptr()] if momentum else []))
+  if min(b - a for a, b in zip(at, at[1:])) < 4 * n:
     raise ValueError("clipped_sgd_momentum_l2: buffers overlap")
   if skip is not None and (skip.dtype != torch.float32 or skip.numel() < 2 or skip.device != params.device
                            or not skip.is_contiguous()):

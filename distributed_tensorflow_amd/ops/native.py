@@ -115,6 +115,7 @@ def clip_list_build(table, at: List[int], to: List[int], kept: bool):
       with torch.cuda.device(table.device):
         # a blocking copy: complete for every stream when it returns
         table.resident = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(table.device)
+        table.held.append(table.resident)
         table.stream = _current_stream(table.device.index)
 
 

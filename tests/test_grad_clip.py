@@ -347,6 +347,92 @@ def test_gpu_one_table_on_two_streams_and_in_two_graphs():
     check_clipped(plain, ts, f)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("name", list(LISTS))
+def test_tables_of_every_list(dev, name):
+  """A table that is kept walks its list from device memory where the arguments of one launch do not hold it; out of
+  place, in place and from one call to the next."""
+  ts = values(*LISTS[name], dev, seed=3)
+  outs = [torch.empty_like(t) for t in ts]
+  kept, inplace = fused.TensorTable(ts, out=outs), fused.TensorTable(ts)
+  if dev == "cuda":
+    full = sum(n > 0 for n in LISTS[name][0])
+    assert (kept.resident is not None) == (full > 120)
+  want = norm64(ts)
+  for clip in (0.05, 1e9):
+    check_norm(fused.global_norm(kept), want)
+    _, norm = fused.clip_by_global_norm(kept, clip)
+    check_norm(norm, want)
+    check_clipped(outs, ts, min(1.0, clip / want) if want else 1.0)
+  given = torch.tensor(10.0, device=dev)
+  fused.clip_by_global_norm(kept, 5.0, use_norm=given)
+  check_clipped(outs, ts, 0.5)
+  keep = [t.clone() for t in ts]
+  _, norm = fused.clip_by_global_norm(inplace, 0.05)
+  check_norm(norm, want)
+  check_clipped(ts, keep, min(1.0, 0.05 / want) if want else 1.0)
+
+
+@pytest.mark.gpu
+def test_gpu_long_table_on_streams_in_graphs_and_after_an_exchange():
+  """A device table is read by two streams and a captured graph; one storage is exchanged afterwards (the graph keeps
+  the table it was captured with), then everything is dropped while work may still be under way."""
+  sizes = [(37 * i) % 3000 + 1 for i in range(300)]
+  ts = values(sizes, [FP, BF] * 150, "cuda")
+  outs = [torch.empty_like(t) for t in ts]
+  table = fused.TensorTable(ts, out=outs)
+  want = norm64(ts)
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    first = [fused.global_norm(table) for _ in range(10)]
+  second = [fused.global_norm(table) for _ in range(10)]
+  torch.cuda.synchronize()
+  for n in first + second:
+    check_norm(n, want)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    _, norm = fused.clip_by_global_norm(table, 0.5)
+    listed, other = fused.clip_by_global_norm(ts, 0.5)
+  for i in range(3):
+    for t in ts:
+      t.mul_(1.25)
+    graph.replay()
+    torch.cuda.synchronize()
+    now = norm64(ts)
+    check_norm(norm, now)
+    check_norm(other, now)
+    check_clipped(outs, ts, 0.5 / now)
+    check_clipped(listed, ts, 0.5 / now)
+  before, before_out = ts[0].data, outs[0].data           # kept alive: the graph still uses them
+  ts[0].data, outs[0].data = torch.ones(9, device="cuda"), torch.zeros(9, device="cuda")
+  _, n = fused.clip_by_global_norm(table, 0.5)
+  now = norm64(ts)
+  check_norm(n, now)
+  check_clipped(outs, ts, 0.5 / now)
+  graph.replay()
+  torch.cuda.synchronize()
+  check_norm(norm, norm64([before] + ts[1:]))
+  with torch.cuda.stream(side):
+    last = fused.global_norm(table)
+  del table
+  fill = [torch.full((1 << 18,), 3.0, device="cuda") for _ in range(8)]
+  torch.cuda.synchronize()
+  check_norm(last, now)
+  assert len(fill) == 8 and before_out.numel() == sizes[0]
+
+
+@pytest.mark.gpu
+def test_gpu_more_than_two_to_the_31_elements():
+  n = (1 << 31) + 4099
+  t = torch.ones(n, dtype=BF, device="cuda")
+  check_norm(fused.global_norm([t]), math.sqrt(n))
+  t[-1] = 256.0
+  _, norm = fused.clip_by_global_norm([t], math.sqrt(n + 65535) / 2, out=[t])
+  check_norm(norm, math.sqrt(n + 65535))
+  assert (t[-5000:-1] == 0.5).all() and float(t[-1]) == 128.0 and float(t[0]) == 0.5 and float(t[1 << 30]) == 0.5
+
+
 @pytest.mark.gpu
 def test_gpu_update_captured_in_a_graph():
   gen = torch.Generator().manual_seed(9)

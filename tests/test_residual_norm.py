@@ -429,6 +429,54 @@ def test_gpu_same_bits_every_time_and_nothing_behind_the_rows(rows, channels, ga
     assert torch.equal(got[:n].view(rows, channels), w) and (got[n:] == 7.0).all()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("channels", [16, 24, 136, 512, 640, 1032, 4096])
+@pytest.mark.parametrize("gate,act", [("none", "none"), ("element", "sigmoid"), ("group", "none")])
+def test_infinities_and_nans_stay_in_their_row_of_whole_chunks(dev, channels, gate, act):
+  """Rows of whole chunks read their last chunk again in the lanes behind it: bad values there reach no other row, and
+  no sum over rows but their own channel's."""
+  rows = 21
+  t, kw = make(dev, rows, channels, torch.bfloat16, "layer", gate=gate, groups=7)
+  kw["gate_act"] = act
+  clean = fused.residual_norm(t["x"], t["y"], **kw)
+  clean_g = fused.residual_norm_grad(t["dh"], t["dz"], t["x"], t["y"], **kw)
+  for n in ("x", "y", "dh", "dz"):
+    t[n][rows - 1, -1] = float("inf")
+    t[n][rows - 2, -2] = float("nan")
+  good = list(range(rows - 2))
+  for a, b in zip(clean, fused.residual_norm(t["x"], t["y"], **kw)):
+    assert torch.equal(a[good], b[good])
+  g = fused.residual_norm_grad(t["dh"], t["dz"], t["x"], t["y"], **kw)
+  for n in ("dx", "dy"):
+    assert torch.equal(clean_g[n][good], g[n][good])
+  if gate == "group":
+    assert torch.equal(clean_g["dgate"][:6], g["dgate"][:6])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,channels", [(4_200_000, 512), (2_150_000, 1001), (265_000, 8192)])
+def test_gpu_offsets_past_32_bits(rows, channels):
+  """More than 2^31 elements a tensor: the last rows as a call on them alone gives them."""
+  z = lambda: torch.zeros(rows, channels, dtype=torch.bfloat16, device="cuda")
+  t, kw = make("cuda", 64, channels, torch.bfloat16, "rms", gate="group", groups=1)
+  big = {n: z() for n in t}
+  for n in t:
+    big[n][-64:] = t[n]
+  want = fused.residual_norm(t["x"], t["y"], **kw)
+  got = fused.residual_norm(big["x"], big["y"], **kw)
+  for a, b in zip(want, got):
+    assert torch.equal(a, b[-64:]) and not b[:64].any()
+  del got
+  want = fused.residual_norm_grad(t["dh"], t["dz"], t["x"], t["y"], **kw)
+  got = fused.residual_norm_grad(big["dh"], big["dz"], big["x"], big["y"], **kw)
+  for n, a in want.items():
+    if a is not None and n in ("dx", "dy"):
+      assert torch.equal(a, got[n][-64:]) and not got[n][:64].any()
+    elif a is not None:      # the same 64 terms of a column in other places of the sum; a term is under 16 (|dz| + |dh|)
+      terms = 16 * (t["dz"].float().abs().sum(0) + t["dh"].float().abs().sum(0))
+      assert ((a - got[n]).abs() <= 64 * U * terms).all(), n
+
+
 @pytest.mark.gpu
 def test_gpu_captured_and_replayed():
   """Two captures of the same calls, replayed in turn with eager work between, new values in the same buffers."""
