@@ -13,11 +13,14 @@
 // A norm that is infinite or NaN makes every result NaN, as TensorFlow's clip_by_global_norm has it; a norm of zero
 // leaves the gradients alone.
 //
-// Tensors are cut into chunks of 16 KB that never cross a tensor; the blocks walk the chunks side by side, two blocks
-// a CU (a narrow front over the memory: a read of 411 MB runs at 7.2 TB/s with 512 blocks, at 5.9 with 2048).  Which
-// tensor a chunk belongs to is looked up while the chunk before it is loaded: in a table in the kernel's arguments (a
-// list given as such: nothing to upload and keep alive, and a captured launch holds its own copy), or in device memory
-// (a table that is kept: any number of tensors in one launch).
+// Tensors are cut into chunks of 8 KB that never cross a tensor; the blocks walk the chunks side by side, four blocks a CU
+// (a narrow front over the memory; 400 M mixed elements: 419 us, chunks of 16 KB 436, of 4 KB 545; with runs of chunks of
+// each block's own 538).  Which tensor a chunk belongs to is looked up while the chunk before it is loaded: in a table in the
+// kernel's arguments (a list given as such: nothing to upload and keep alive, and a captured launch holds its own copy), or
+// in device memory (a table that is kept: any number of tensors in one launch).
+//
+// Measured: 161 tensors of 25.6 M fp32 elements 18 + 35 us (5.7 and 5.9 TB/s), 384 of 400 M mixed ones 122 + 295 us (6.6 and
+// 5.5 TB/s); what bounds both is memory, and that the norm has to be known before the first element can be scaled.
 #include <algorithm>
 #include <stdexcept>
 
@@ -26,8 +29,10 @@
 namespace {
 
 constexpr int TPB = 256;
-constexpr int CHUNK_BYTES = TPB * 16 * 4;
-constexpr int MAX_BLOCKS = 512;                    // per launch: two a CU
+constexpr int U = 2;          // accesses of 16 bytes a thread and chunk
+constexpr int CHUNK_BYTES = TPB * 16 * U;
+constexpr int MAX_BLOCKS = 1024;                   // per launch: four a CU
+constexpr int SGD_BLOCKS = 512;                    // of the update's two sweeps
 constexpr int64_t CACHE_BYTES = 192 << 20;         // of what a sweep leaves in the memory-side cache (256 MB)
 
 typedef u32x4 __attribute__((aligned(2))) Any16;   // any address will do
@@ -111,21 +116,21 @@ struct Resident {       // a table in device memory
   __device__ __forceinline__ ClipEntry at(uint32_t c) const { return e[map[c]]; }
 };
 
-// A thread's four pieces of 16 bytes of a chunk; past the tensor's end: zeros.
+// A thread's pieces of 16 bytes of a chunk; past the tensor's end: zeros.
 template <bool NT>
 __device__ __forceinline__ void load_chunk(const ClipEntry& e, uint32_t c, u32x4* v) {
   const int64_t at = (int64_t)(c - e.first) * CHUNK_BYTES + (int64_t)threadIdx.x * 16;
   const char* p = reinterpret_cast<const char*>(e.in);
   if (at - (int64_t)threadIdx.x * 16 + CHUNK_BYTES <= e.bytes) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < U; ++k) {
       const Any16* q = reinterpret_cast<const Any16*>(p + at + k * TPB * 16);
       if constexpr (NT) v[k] = __builtin_nontemporal_load(q);
       else v[k] = *q;
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < U; ++k) {
       const int64_t o = at + k * TPB * 16;
       v[k] = u32x4{0u, 0u, 0u, 0u};
       if (o + 16 <= e.bytes) {
@@ -144,7 +149,7 @@ __device__ __forceinline__ void store_chunk(const ClipEntry& e, uint32_t c, cons
   const int64_t at = (int64_t)(c - e.first) * CHUNK_BYTES + (int64_t)threadIdx.x * 16;
   char* p = reinterpret_cast<char*>(e.out);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < U; ++k) {
     const int64_t o = at + k * TPB * 16;
     if (o + 16 <= e.bytes) {
       Any16* q = reinterpret_cast<Any16*>(p + o);
@@ -161,7 +166,7 @@ __device__ __forceinline__ void store_chunk(const ClipEntry& e, uint32_t c, cons
 template <int DT>
 __device__ __forceinline__ void add_squares(const u32x4* v, double* s) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < U; ++k) {
     float f[8];
     const int n = unpack<DT>(v[k], f);
 #pragma unroll
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(TPB) void norm_kernel(const T t, uint32_t cold, dou
   ClipEntry e = {};
   if (c < chunks) e = t.at(c);
   while (c < chunks) {
-    u32x4 v[4];
+    u32x4 v[U];
     if (c < cold) load_chunk<true>(e, c, v);
     else load_chunk<false>(e, c, v);
     const int dt = e.dt;
@@ -214,12 +219,12 @@ __global__ __launch_bounds__(TPB) void scale_kernel(const T t, const double* __r
   while (k < chunks) {
     const ClipEntry e = next;
     const uint32_t c = chunks - 1 - k;
-    u32x4 v[4];
+    u32x4 v[U];
     load_chunk<false>(e, c, v);
     k += gridDim.x;
     if (k < chunks) next = t.at(chunks - 1 - k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < U; ++i)
       v[i] = e.dt == DT_BF16 ? scaled<DT_BF16>(v[i], factor) : e.dt == DT_F16 ? scaled<DT_F16>(v[i], factor)
                                                                                : scaled<DT_F32>(v[i], factor);
     if (nt) store_chunk<true>(e, c, v);
@@ -334,7 +339,7 @@ ClipList::ClipList(const std::vector<uintptr_t>& in, const std::vector<uintptr_t
     e.dt = dt[i];
     e.first = (uint32_t)chunks_;
     chunks_ += ((uint64_t)e.bytes + CHUNK_BYTES - 1) / CHUNK_BYTES;
-    if (chunks_ > 0x7fffffffull) throw std::invalid_argument("a list of up to 32 TB");
+    if (chunks_ > 0x7fffffffull) throw std::invalid_argument("a list of up to 16 TB");
     bytes_ += e.bytes;
     in_place_ = in_place_ && e.in == e.out;
     outputs_ = outputs_ && e.out;
@@ -426,7 +431,7 @@ void ClipList::scale(const void* resident, const double* ws, const float* use_no
 
 int clipped_sgd_blocks(size_t n) {
   const size_t want = (n / 4 + TPB - 1) / TPB;
-  return (int)std::min<size_t>(std::max<size_t>(want, 1), MAX_BLOCKS);
+  return (int)std::min<size_t>(std::max<size_t>(want, 1), SGD_BLOCKS);
 }
 
 void launch_clipped_sgd_momentum_l2(float* p, const float* g, float* v, const float* l2x2, size_t n, float lr,
