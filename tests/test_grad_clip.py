@@ -546,3 +546,72 @@ def test_training_step_of_a_residual_stack(dev, norm):
     assert (params.double().cpu() - p64).abs().max() <= 1e-4 * lr * clip * 2
     # the next step starts from the same parameters on both sides
     p64, v64 = params.double().cpu(), vel.double().cpu()
+
+
+def test_driver_run_with_the_flag(tmp_path, monkeypatch):
+  """A CIFAR driver run whose updates are clipped so far that the variables hardly move, against one that is not."""
+  import os
+  import sys
+  root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+  if root not in sys.path:
+    sys.path.insert(0, root)
+  import resnet_cifar_main
+  from distributed_tensorflow_amd.train.model import Model
+  from distributed_tensorflow_amd.utils import flags as flags_core
+  for k in ("RANK", "WORLD_SIZE", "LOCAL_RANK", "TF_CONFIG"):
+    monkeypatch.delenv(k, raising=False)
+  seen = []
+  fit = Model.fit
+
+  def watched(self, *a, **k):
+    before = self.store.params.clone()
+    out = fit(self, *a, **k)
+    seen.append((self.optimizer, float((self.store.params - before).norm()), int(self.optimizer.iterations)))
+    return out
+
+  monkeypatch.setattr(Model, "fit", watched)
+  resnet_cifar_main.define_cifar_flags()
+  common = [sys.argv[0], "--train_steps", "2", "--use_synthetic_data", "--num_gpus", "0", "--batch_size", "4",
+            "--distribution_strategy", "off", "--skip_eval", "--model_dir", str(tmp_path)]
+  for more in ([], ["--global_clipnorm", "1e-6"]):
+    flags_core.FLAGS.unparse_flags()
+    flags_core.FLAGS(common + more)
+    resnet_cifar_main.run(flags_core.FLAGS)
+  (plain, moved, _), (clipped, held, steps) = seen
+  assert plain.global_clipnorm is None and clipped.global_clipnorm == 1e-6
+  assert float(clipped.gradient_norm) > 1e-6
+  # a step moves by at most rate * clip, momentum adds up to steps * (steps + 1) / 2 of them; the rate is at most 0.1
+  # and fp32 variables of norm under 100 round by 2^-24 of it an update
+  assert held <= 0.1 * 1e-6 * steps * (steps + 1) / 2 + steps * 100 * U < moved
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,scale", [("bf16", None), ("fp16", "dynamic")])
+def test_gpu_training_steps_with_the_clipped_optimizer(dtype, scale):
+  """The native engine with SGD(global_clipnorm=): every step is the update of the engine's own gradients in 64 bits,
+  with the loss scale's factor taken from the device where scaling is dynamic; an infinite gradient leaves the step out."""
+  from distributed_tensorflow_amd.train.model import Model
+  m = Model(models.resnet20(), dtype=dtype, device=torch.device("cuda"), seed=3, deterministic=True)
+  opt = SGD(0.05, momentum=0.9, global_clipnorm=0.1)
+  wrapped = opt if scale is None else LossScaleOptimizer(opt, scale, initial_scale=256.0)
+  m.compile(wrapped, "sparse_categorical_crossentropy")
+  g = torch.Generator().manual_seed(0)
+  x = (torch.randn(8, 32, 32, 3, generator=g) * 50 + 100).cuda()
+  y = torch.randint(0, 10, (8, 1), generator=g).float().cuda()
+  st = m.store
+  for _ in range(3):
+    before = [t.double().cpu().clone() for t in (st.params, st.slot("momentum"))]
+    m.train_on_batch(x, y)
+    factor = 1.0 if scale is None else float(wrapped._dev_state[4])
+    p, v, norm, size = update64(before[0], st.grads.double().cpu(), before[1], st.l2_vector().double().cpu(), 0.05, 0.9,
+                                0.1, factor)
+    assert norm > 0.1 and abs(float(opt.gradient_norm) - norm) <= 4 * U * norm
+    assert ((st.slot("momentum").double().cpu() - v).abs() <= 12 * U * (size + v.abs())).all()
+    assert ((st.params.double().cpu() - p).abs() <= 12 * U * (size + v.abs()) + 2 * U * p.abs()).all()
+  if scale:
+    keep = st.params.clone(), st.slot("momentum").clone()
+    st.grads[7] = float("inf")
+    skipped = wrapped.skipped_steps
+    wrapped.apply_gradients(st, 1.0, m._executor(8))
+    assert wrapped.skipped_steps == skipped + 1
+    assert torch.equal(st.params, keep[0]) and torch.equal(st.slot("momentum"), keep[1])
