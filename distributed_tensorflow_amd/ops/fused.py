@@ -349,7 +349,7 @@ def _squares(tensors) -> torch.Tensor:
 def global_norm(tensors) -> torch.Tensor:
   """sqrt of the sum of squares over all tensors of a list or `TensorTable`: a float32 scalar on their device.
 
-  Squares are summed in 64 bits in a fixed order; nothing is read back to the host.
+  Squares are summed in 64 bits in a fixed order; nothing is read back to the host, and no graph is recorded.
   """
   t = _table(tensors)
   if t.device.type != "cuda":
