@@ -1,4 +1,4 @@
-"""Builds the native extension `_dtf_native` for gfx950 with hipcc (no torch headers needed).
+"""Builds the native extension `_dtf_native` for gfx950 with hipcc (of torch only the header of DLPack's C structures).
 
     python -m distributed_tensorflow_amd.ops.build [--force] [--jobs N]
 
@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures
+import importlib.util
 import os
 import subprocess
 import sys
@@ -32,7 +33,7 @@ HEADERS = ["common.h", "conv_params.h", "conv_epilogue.h", "elementwise.h", "rcc
 _RESIDUAL_NORM = ["residual_norm.h", "residual_norm_kernels.h"]
 OWN_HEADERS = {"residual_norm.hip": _RESIDUAL_NORM, "residual_norm_bf16.hip": _RESIDUAL_NORM,
                "residual_norm_f16.hip": _RESIDUAL_NORM, "residual_norm_f32.hip": _RESIDUAL_NORM,
-               "grad_clip.hip": ["grad_clip.h"], "bindings.cpp": ["residual_norm.h", "grad_clip.h"]}
+               "grad_clip.hip": ["grad_clip.h"], "bindings.cpp": ["residual_norm.h", "grad_clip.h", "tensor_keys.h"]}
 
 
 def so_path() -> str:
@@ -41,7 +42,9 @@ def so_path() -> str:
 
 def _includes():
   import pybind11  # pylint: disable=import-outside-toplevel
-  return ["-I" + sysconfig.get_paths()["include"], "-I" + pybind11.get_include(), "-I" + CSRC]
+  torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+  return ["-I" + sysconfig.get_paths()["include"], "-I" + pybind11.get_include(), "-I" + CSRC,
+          "-I" + os.path.join(torch, "include")]
 
 
 def _stale(target, deps):

@@ -26,6 +26,7 @@
 #include "grad_clip.h"
 #include "rccl_comm.h"
 #include "residual_norm.h"
+#include "tensor_keys.h"
 
 namespace py = pybind11;
 using Launch = std::function<void(hipStream_t)>;
@@ -859,6 +860,10 @@ PYBIND11_MODULE(_dtf_native, m) {
     check_launch();
   });
   m.attr("RESIDUAL_NORM_MAX_C") = RESIDUAL_NORM_MAX_C;
+  m.def("tensor_keys", [](const py::list& tensors) -> py::object {
+    return TensorKeys::available() ? py::cast(TensorKeys(tensors)) : py::none();
+  }, "Keys of a list of tensors; None where this torch does not hand its tensors out to C");
+  py::class_<TensorKeys>(m, "TensorKeys").def("same", &TensorKeys::same);
   py::class_<ClipList>(m, "ClipList")
       .def(py::init<const std::vector<uintptr_t>&, const std::vector<uintptr_t>&, const std::vector<int64_t>&,
                     const std::vector<int>&>(), py::arg("in"), py::arg("out"), py::arg("n"), py::arg("dt"))

@@ -277,9 +277,10 @@ class TensorTable:
   same buffers step after step (a plan, like the launch plan of a training step).
 
   `out`: where clipped tensors go, a list of the same shapes and types (the tensors themselves: in place); without
-  it they are clipped in place.  The table keeps the tensors alive and follows them: one whose storage was exchanged
-  since is looked up again by the next call.  Keep the table itself for as long as a graph that was captured with it.  Contiguous bfloat16, float16 or float32 tensors of one device; outputs may
-  not overlap each other, nor any input but their own.
+  it they are clipped in place.  The table keeps the tensors alive and follows them: one whose storage, length, type or
+  layout was exchanged since is looked up again, and checked again, by the next call.  Keep the table itself for as long
+  as a graph that was captured with it.  Contiguous bfloat16, float16 or float32 tensors of one device; outputs may not
+  overlap each other, nor any input but their own.
   """
 
   def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None, *, _kept=True):
@@ -304,8 +305,8 @@ class TensorTable:
         raise ValueError("tensor %d is not contiguous" % i)
       if o.shape != t.shape or o.dtype != t.dtype:
         raise ValueError("output %d: %s %s for %s %s" % (i, tuple(o.shape), o.dtype, tuple(t.shape), t.dtype))
-    self._at = [t.data_ptr() for t in self.tensors]
-    self._to = self._at if self.out is self.tensors else [o.data_ptr() for o in self.out]
+    at = [t.data_ptr() for t in self.tensors]
+    to = at if self.out is self.tensors else [o.data_ptr() for o in self.out]
     # refused by clip_by_global_norm alone: a norm may count a tensor twice
     outs = [_span(o) for o in self.out]
     apart = [_span(t) for t, o in zip(self.tensors, self.out) if t.data_ptr() != o.data_ptr()]
@@ -314,13 +315,40 @@ class TensorTable:
     self.list, self.workspace, self.resident, self.stream = None, 0, None, 0
     if self.device.type == "cuda":
       from . import native  # pylint: disable=import-outside-toplevel
-      native.clip_list_build(self, self._at, self._to, self._kept)
+      native.clip_list_build(self, at, to, self._kept)
+    # last: a build that raises leaves the table as changed as it found it
+    self._keys = [self._keys_of(ts) for ts in self._lists()]
+
+  def _lists(self):
+    return (self.tensors,) if self.out is self.tensors else (self.tensors, self.out)
+
+  def _keys_of(self, tensors):
+    """What the launches depend on of every tensor: address, length, type, order of its elements."""
+    if self.device.type == "cuda":
+      from . import native  # pylint: disable=import-outside-toplevel
+      keys = native.ext().tensor_keys(tensors)
+      if keys is not None:
+        return keys
+    return _Keys(tensors)
 
   def _current(self) -> "TensorTable":
-    if self._at != list(map(torch.Tensor.data_ptr, self.tensors)) or (
-        self.out is not self.tensors and self._to != list(map(torch.Tensor.data_ptr, self.out))):
+    if not all(k.same(ts) for k, ts in zip(self._keys, self._lists())):
       self._build()
     return self
+
+
+class _Keys:
+  """Keys of a list of tensors by their attributes (`TensorKeys` of the native extension is the fast form)."""
+
+  def __init__(self, tensors):
+    self._keys = self._read(tensors)
+
+  @staticmethod
+  def _read(tensors):
+    return [(t.data_ptr(), t.numel(), t.dtype, t.is_contiguous()) for t in tensors]
+
+  def same(self, tensors) -> bool:
+    return self._keys == self._read(tensors)
 
 
 def _overlaps_two(a, b) -> bool:

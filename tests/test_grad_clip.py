@@ -615,3 +615,102 @@ def test_gpu_training_steps_with_the_clipped_optimizer(dtype, scale):
     wrapped.apply_gradients(st, 1.0, m._executor(8))
     assert wrapped.skipped_steps == skipped + 1
     assert torch.equal(st.params, keep[0]) and torch.equal(st.slot("momentum"), keep[1])
+
+
+def _change(t, how):
+  """The tensor with its data exchanged for something else at the same address."""
+  flat = t.data.view(-1)
+  if how == "shorter":
+    t.data = flat[:1000]
+  elif how == "longer":
+    t.data = flat.as_strided((6000,), (1,))
+  elif how == "another type":
+    t.data = flat.view(HF)
+  elif how == "resized":
+    t.resize_(7, 11)
+  else:
+    t.t_()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("count", [1, 130])
+@pytest.mark.parametrize("how", ["shorter", "longer", "another type", "resized"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_table_follows_what_changes_at_the_same_address(dev, count, how, in_place):
+  """Length and type belong to what a table goes by: with the address as it was, exactly the tensor's present elements are
+  normed and clipped, as its present type; nothing else of the memory is touched.  130: walked from device memory."""
+  base = values([8192, 8192], [BF, BF], dev, seed=5)
+  rest = values([50] * (count - 1), [FP] * (count - 1), dev, seed=6)
+  ts = [base[0][:3000].view(60, 50)] + rest
+  outs = ts if in_place else [base[1][:3000].view(60, 50)] + [torch.empty_like(t) for t in rest]
+  table = fused.TensorTable(ts) if in_place else fused.TensorTable(ts, out=outs)
+  fused.clip_by_global_norm(table, 1e9)
+  at = ts[0].data_ptr()
+  keep = [b.clone() for b in base]
+  _change(ts[0], how)
+  if not in_place:
+    # an output that no longer fits is refused, before anything runs
+    with pytest.raises(ValueError, match="output 0"):
+      fused.clip_by_global_norm(table, 1.0)
+    with pytest.raises(ValueError, match="output 0"):
+      fused.global_norm(table)
+    _change(outs[0], how)
+  assert ts[0].data_ptr() == at
+  want = norm64(ts)
+  inputs = [t.clone() for t in ts]
+  check_norm(fused.global_norm(table), want)
+  got, norm = fused.clip_by_global_norm(table, want / 4)
+  check_norm(norm, want)
+  check_clipped(got, inputs, float(torch.tensor(want / 4, dtype=torch.float32)) / want)
+  n = ts[0].numel()
+  assert all(torch.equal(b[n:].view(torch.int16), k[n:].view(torch.int16)) for b, k in zip(base, keep))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_table_refuses_a_tensor_that_was_transposed_or_left_its_types(dev):
+  ts = [torch.randn(40, 50, device=dev), torch.randn(9, device=dev)]
+  outs = [torch.empty_like(t) for t in ts]
+  table = fused.TensorTable(ts, out=outs)
+  check_norm(fused.global_norm(table), norm64(ts))
+  ts[0].t_()
+  for _ in range(2):        # a refusal leaves the table as it was: the next call is refused too
+    with pytest.raises(ValueError, match="tensor 0 is not contiguous"):
+      fused.clip_by_global_norm(table, 1.0)
+  ts[0].t_()
+  want = norm64(ts)
+  check_clipped(fused.clip_by_global_norm(table, 0.5)[0], ts, 0.5 / want)
+  outs[0].t_()
+  with pytest.raises(ValueError, match="contiguous"):
+    fused.clip_by_global_norm(table, 1.0)
+  outs[0].t_()
+  ts[1].data = torch.randn(18, device=dev).view(torch.float64)
+  with pytest.raises(ValueError, match="element type"):
+    fused.global_norm(table)
+
+
+def test_keys_of_tensors():
+  """The native keys say what the attributes say, of every kind of change."""
+  from distributed_tensorflow_amd.ops import native
+  if not native.available():
+    pytest.skip("no native extension")
+  base = torch.zeros(4096)
+  make = {
+      "same": lambda t: None, "values": lambda t: t.add_(1), "address": lambda t: setattr(t, "data", base[1:601].view(20, 30)),
+      "length": lambda t: setattr(t, "data", base[:570].view(19, 30)), "type": lambda t: setattr(t, "data", t.view(torch.int32)),
+      "narrower type": lambda t: setattr(t, "data", base[:300].view(HF).view(20, 30)), "transposed": lambda t: t.t_(),
+      "shape": lambda t: setattr(t, "data", t.view(1, 600, 1)), "pitch": lambda t: setattr(t, "data", base.as_strided((20, 30), (60, 1))),
+      "one row, any pitch": lambda t: setattr(t, "data", base.as_strided((1, 600), (7, 1))), "empty": lambda t: t.resize_(0),
+      "gradient": lambda t: t.requires_grad_(True), "resized": lambda t: t.resize_(3, 3)}
+  for what, change in make.items():
+    ts = [torch.zeros(3), base[:600].view(20, 30), torch.zeros(()), torch.zeros(0, 5)]
+    slow, fast = fused._Keys(ts), native.ext().tensor_keys(ts)
+    if fast is None:
+      pytest.skip("this torch does not hand its tensors out to C")
+    assert slow.same(ts) and fast.same(ts)
+    change(ts[1])
+    same = what in ("same", "values", "shape", "one row, any pitch", "gradient")
+    assert slow.same(ts) == same and fast.same(ts) == same, what
+    assert not fast.same(ts[:3]) and not slow.same(ts[:3])
+  assert not native.ext().tensor_keys([base]).same([None])
+  with pytest.raises(ValueError):
+    native.ext().tensor_keys([3])
