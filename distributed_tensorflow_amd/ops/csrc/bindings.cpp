@@ -870,6 +870,7 @@ PYBIND11_MODULE(_dtf_native, m) {
       .def("table", [](const ClipList& l) { return py::bytes(l.table()); },
            "What `resident` points to in device memory; empty where the arguments of one launch hold the list")
       .def_property_readonly("workspace_doubles", &ClipList::workspace_doubles)
+      .def_property_readonly("pieces", &ClipList::pieces)
       .def("global_norm", [](const ClipList& l, uintptr_t resident, uintptr_t ws, uintptr_t norm, uintptr_t stream) {
              auto* w = reinterpret_cast<double*>(ws);
              auto* r = reinterpret_cast<const void*>(resident);

@@ -21,6 +21,7 @@ class ClipList {
            const std::vector<int>& dt);
   // What `resident` has to point to: the entries, then a chunk's entry for every chunk.  Empty: one launch does anyway.
   std::string table() const;
+  size_t pieces() const { return pieces_.size(); }      // launches of a sweep without `resident`
   size_t workspace_doubles() const { return partials_; }
   void norm(const void* resident, double* ws, hipStream_t s) const;                  // partial sums of squares
   void finish(const void* resident, const double* ws, float* norm, hipStream_t s) const;

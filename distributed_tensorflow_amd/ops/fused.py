@@ -292,10 +292,10 @@ class TensorTable:
     if len(self.out) != len(self.tensors):
       raise ValueError("%d outputs for %d tensors" % (len(self.out), len(self.tensors)))
     self.device = self.tensors[0].device
-    self.held = []          # every device table written so far: a captured graph may still read an older one
-    self._build()
+    self.held = []          # device tables that a captured graph reads, now and after an exchange of storages
+    self._build(self._kept)
 
-  def _build(self):
+  def _build(self, upload):
     for i, (t, o) in enumerate(zip(self.tensors, self.out)):
       if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("tensor %d: element type %s (bfloat16, float16 and float32 are built)" % (i, t.dtype))
@@ -313,9 +313,13 @@ class TensorTable:
     self._clash = _overlaps(outs) or (bool(apart) and _overlaps_two(outs, apart))
     # native: the launches, the doubles they need, their table in device memory and the stream it was written on
     self.list, self.workspace, self.resident, self.stream = None, 0, None, 0
+    self._upload_due = False
     if self.device.type == "cuda":
       from . import native  # pylint: disable=import-outside-toplevel
-      native.clip_list_build(self, at, to, self._kept)
+      native.clip_list_build(self, at, to)
+      self._upload_due = self._kept and self.list.pieces > 1
+      if upload:
+        self._upload()
     # last: a build that raises leaves the table as changed as it found it
     self._keys = [self._keys_of(ts) for ts in self._lists()]
 
@@ -331,9 +335,17 @@ class TensorTable:
         return keys
     return _Keys(tensors)
 
+  def _upload(self):
+    from . import native  # pylint: disable=import-outside-toplevel
+    self._upload_due = self._upload_due and not native.clip_list_upload(self)
+
   def _current(self) -> "TensorTable":
+    # a list that changed is walked from launch arguments; its table goes to the device once a call finds it unchanged,
+    # so that storages that are exchanged at every step neither pile up tables nor wait for their upload
     if not all(k.same(ts) for k, ts in zip(self._keys, self._lists())):
-      self._build()
+      self._build(upload=False)
+    elif self._upload_due:
+      self._upload()
     return self
 
 

@@ -18,8 +18,7 @@ except ImportError as e:                      # pragma: no cover - exercised onl
   _import_error = e
 
 __all__ = ["available", "ext", "run_op", "Plan", "stream_handle", "sgd_momentum_l2", "loss_scale_step",
-           "clipped_sgd_momentum_l2", "clip_list_build", "clip_list_norm",
-           "clip_list_scale",
+           "clipped_sgd_momentum_l2", "clip_list_build", "clip_list_upload", "clip_list_norm", "clip_list_scale",
            "residual_norm", "residual_norm_grad", "dtype_code", "pack_desc_bytes", "pack_blocks", "PACK_PER_BLOCK"]
 
 PACK_PER_BLOCK = 256 * 8
@@ -103,30 +102,37 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
   return norm
 
 
-def clip_list_build(table, at: List[int], to: List[int], kept: bool):
-  """Native half of a `fused.TensorTable`.  One that is kept and does not fit the arguments of a launch gets a table in
-  device memory (not while a graph is captured: an upload would become part of it)."""
+def clip_list_build(table, at: List[int], to: List[int]):
+  """Native half of a `fused.TensorTable`."""
   ts = table.tensors
   table.list = ext().ClipList(at, to, [t.numel() for t in ts], [dtype_code(t.dtype) for t in ts])
   table.workspace = max(table.list.workspace_doubles, 1)
-  if kept and not torch.cuda.is_current_stream_capturing():
-    raw = table.list.table()
-    if raw:
-      with torch.cuda.device(table.device):
-        # a blocking copy: complete for every stream when it returns
-        table.resident = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(table.device)
-        table.held.append(table.resident)
-        table.stream = _current_stream(table.device.index)
+
+
+def clip_list_upload(table) -> bool:
+  """Writes the list to device memory, where one launch walks any number of tensors; False while a graph is captured (the
+  upload would become part of it)."""
+  with torch.cuda.device(table.device):
+    if torch.cuda.is_current_stream_capturing():
+      return False
+    # a blocking copy: complete for every stream when it returns
+    table.resident = torch.frombuffer(bytearray(table.list.table()), dtype=torch.uint8).to(table.device)
+    table.stream = _current_stream(table.device.index)
+  return True
 
 
 def _clip_list_launch(table, stream: int):
   """(address of the device table or 0, norm, workspace) of a call.  The workspace is the call's own: tables are shared
-  between streams.  The device table is held back from reuse until a foreign stream is done with it."""
+  between streams.  The device table is held back from reuse until a foreign stream is done with it, and for good once
+  a graph has captured it."""
   dev = table.device
   resident = 0
   if table.resident is not None:
     resident = table.resident.data_ptr()
-    if stream != table.stream:
+    if torch.cuda.is_current_stream_capturing():
+      if not any(r is table.resident for r in table.held):
+        table.held.append(table.resident)
+    elif stream != table.stream:
       table.resident.record_stream(torch.cuda.current_stream(dev))
   return (resident, torch.empty((), dtype=torch.float32, device=dev),
           torch.empty(table.workspace, dtype=torch.float64, device=dev))

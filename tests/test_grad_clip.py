@@ -714,3 +714,42 @@ def test_keys_of_tensors():
   assert not native.ext().tensor_keys([base]).same([None])
   with pytest.raises(ValueError):
     native.ext().tensor_keys([3])
+
+
+@pytest.mark.gpu
+def test_gpu_storages_exchanged_at_every_step():
+  """No device table is kept of a list that changes from call to call; one that settles is walked from device memory
+  again, and one that a graph has captured stays for the graph."""
+  sizes = [(53 * i) % 2000 + 1 for i in range(200)]
+  ts = values(sizes, [FP, BF] * 100, "cuda")
+  table = fused.TensorTable(ts)
+  assert table.resident is not None
+  stream = torch.cuda.Stream()
+  for step in range(5):
+    for i in (0, 7, 199):
+      ts[i].data = values([sizes[i] + step], [ts[i].dtype], "cuda", seed=step)[0]
+    want = norm64(ts)
+    keep = [t.clone() for t in ts]
+    _, norm = fused.clip_by_global_norm(table, want / 2)
+    check_norm(norm, want)
+    check_clipped(ts, keep, float(torch.tensor(want / 2, dtype=torch.float32)) / want)
+    assert table.resident is None and not table.held
+  check_norm(fused.global_norm(table), norm64(ts))
+  assert table.resident is not None and not table.held
+  graph = torch.cuda.CUDAGraph()
+  stream.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.graph(graph, stream=stream):
+    first, second = fused.global_norm(table), fused.global_norm(table)
+  assert len(table.held) == 1
+  captured = [t.data for t in ts]
+  ts[3].data = torch.ones(5, device="cuda", dtype=ts[3].dtype)
+  check_norm(fused.global_norm(table), norm64(ts))
+  check_norm(fused.global_norm(table), norm64(ts))
+  fill = [torch.full((1 << 16,), 255, dtype=torch.uint8, device="cuda") for _ in range(16)]
+  for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    check_norm(first, norm64(captured))
+    check_norm(second, norm64(captured))
+    captured[0].mul_(1.5)
+  assert len(table.held) == 1 and len(fill) == 16
