@@ -417,7 +417,7 @@ def clip_by_global_norm(tensors, clip_norm: float, use_norm: Optional[torch.Tens
   else:
     tensors = list(tensors)
     t = TensorTable(tensors, [torch.empty_like(x, memory_format=torch.contiguous_format) for x in tensors]
-                    if out is None else out)
+                    if out is None else out, _kept=False)
   if t._clash:
     raise ValueError("outputs overlap each other, or another tensor's input")
   if use_norm is not None and (use_norm.dtype != torch.float32 or use_norm.numel() != 1

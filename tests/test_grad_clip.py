@@ -753,3 +753,26 @@ def test_gpu_storages_exchanged_at_every_step():
     check_norm(second, norm64(captured))
     captured[0].mul_(1.5)
   assert len(table.held) == 1 and len(fill) == 16
+
+
+@pytest.mark.gpu
+def test_gpu_a_list_is_clipped_without_an_upload(monkeypatch):
+  """A list given as such is walked from launch arguments, whatever its length: nothing is copied to the device, so no
+  call waits for the work before it."""
+  from distributed_tensorflow_amd.ops import native
+
+  def refuse(table):
+    raise AssertionError("a table was uploaded")
+
+  ts = values([(29 * i) % 700 + 1 for i in range(500)], [FP, BF] * 250, "cuda")
+  want = norm64(ts)
+  monkeypatch.setattr(native, "clip_list_upload", refuse)
+  outs, norm = fused.clip_by_global_norm(ts, want / 2)
+  check_norm(norm, want)
+  check_clipped(outs, ts, float(torch.tensor(want / 2, dtype=torch.float32)) / want)
+  into = [torch.empty_like(t) for t in ts]
+  fused.clip_by_global_norm(ts, want / 2, out=into)
+  assert all(torch.equal(a, b) for a, b in zip(outs, into))
+  check_norm(fused.global_norm(ts), want)
+  monkeypatch.undo()
+  assert fused.TensorTable(ts).resident is not None
