@@ -26,7 +26,7 @@ class ClipList {
   void norm(const void* resident, double* ws, hipStream_t s) const;                  // partial sums of squares
   void finish(const void* resident, const double* ws, float* norm, hipStream_t s) const;
   // out = in * min(1, clip / norm); the norm comes from `ws`, or from `use_norm` where that is given, and goes to `norm`
-  void scale(const void* resident, const double* ws, const float* use_norm, float clip, float* norm, hipStream_t s) const;
+  void scale(const void* resident, double* ws, const float* use_norm, float clip, float* norm, hipStream_t s) const;
 
   static constexpr int PER_LAUNCH = 120;
   struct Table {        // a kernel argument: under 4 KB
@@ -34,7 +34,6 @@ class ClipList {
     int count;
     uint32_t chunks;
   };
-
 
  private:
   int partials(const void* resident) const;

@@ -321,7 +321,7 @@ class TensorTable:
       if upload:
         self._upload()
     # last: a build that raises leaves the table as changed as it found it
-    self._keys = [self._keys_of(ts) for ts in self._lists()]
+    self._keys = [self._keys_of(ts) for ts in self._lists()] if self._kept else None
 
   def _lists(self):
     return (self.tensors,) if self.out is self.tensors else (self.tensors, self.out)

@@ -776,3 +776,17 @@ def test_gpu_a_list_is_clipped_without_an_upload(monkeypatch):
   check_norm(fused.global_norm(ts), want)
   monkeypatch.undo()
   assert fused.TensorTable(ts).resident is not None
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_list_of_many_launches(dev):
+  """Thirty launches' partial sums, more than one block's share of them, out of place and in place."""
+  sizes = [(7919 * i) % 40_000 + 1 for i in range(3600)]
+  ts = values(sizes, [BF, FP] * 1800, dev, scale=1e-3)
+  want = norm64(ts)
+  outs, norm = fused.clip_by_global_norm(ts, want / 2)
+  check_norm(norm, want)
+  check_norm(fused.global_norm(ts), want)
+  check_clipped(outs, ts, float(torch.tensor(want / 2, dtype=torch.float32)) / want)
+  again, _ = fused.clip_by_global_norm(ts, want / 2, out=ts)
+  assert all(torch.equal(a, b) for a, b in zip(outs, again))
