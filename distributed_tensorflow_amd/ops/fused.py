@@ -308,7 +308,7 @@ class TensorTable:
     at = [t.data_ptr() for t in self.tensors]
     to = at if self.out is self.tensors else [o.data_ptr() for o in self.out]
     # refused by clip_by_global_norm alone: a norm may count a tensor twice
-    outs = [_span(o) for o in self.out]
+    outs = self._out_spans = [_span(o) for o in self.out]
     apart = [_span(t) for t, o in zip(self.tensors, self.out) if t.data_ptr() != o.data_ptr()]
     self._clash = _overlaps(outs) or (bool(apart) and _overlaps_two(outs, apart))
     # native: the launches, the doubles they need, their table in device memory and the stream it was written on
@@ -423,6 +423,8 @@ def clip_by_global_norm(tensors, clip_norm: float, use_norm: Optional[torch.Tens
   if use_norm is not None and (use_norm.dtype != torch.float32 or use_norm.numel() != 1
                                or use_norm.device != t.device):
     raise ValueError("use_norm: a float32 scalar on %s" % t.device)
+  if use_norm is not None and any(lo <= use_norm.data_ptr() < hi for lo, hi in t._out_spans):
+    raise ValueError("use_norm lies in an output: it is read while outputs are written")
   if t.device.type == "cuda":
     from . import native  # pylint: disable=import-outside-toplevel
     return list(t.out), native.clip_list_scale(t, clip_norm, use_norm)
@@ -464,6 +466,9 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
   if skip is not None and (skip.dtype != torch.float32 or skip.numel() < 2 or skip.device != params.device
                            or not skip.is_contiguous()):
     raise ValueError("skip: two contiguous float32 values on %s" % params.device)
+  if skip is not None and any(lo - 8 < skip.data_ptr() < lo + 4 * n
+                              for lo in [params.data_ptr()] + ([velocity.data_ptr()] if momentum else [])):
+    raise ValueError("skip lies in a buffer that is updated: it is read while that is written")
   if params.device.type == "cuda":
     from . import native  # pylint: disable=import-outside-toplevel
     return native.clipped_sgd_momentum_l2(params, grads, velocity, l2x2, lr, momentum, clip_norm, grad_scale, skip)

@@ -790,3 +790,25 @@ def test_list_of_many_launches(dev):
   check_clipped(outs, ts, float(torch.tensor(want / 2, dtype=torch.float32)) / want)
   again, _ = fused.clip_by_global_norm(ts, want / 2, out=ts)
   assert all(torch.equal(a, b) for a, b in zip(outs, again))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_scalars_that_lie_in_an_output_are_refused(dev):
+  """Every block reads the given norm (the skip flag), while others have begun to write."""
+  flat = torch.full((4096,), 2.0, device=dev)
+  keep = flat.clone()
+  for table in (False, True):
+    for at in (0, 1500, 3999):
+      t = fused.TensorTable([flat[:4000]]) if table else [flat[:4000]]
+      with pytest.raises(ValueError, match="use_norm"):
+        fused.clip_by_global_norm(t, 1.0, use_norm=flat[at], **({} if table else dict(out=t)))
+  assert torch.equal(flat, keep)
+  outs, _ = fused.clip_by_global_norm([flat[:4000]], 1.0, use_norm=flat[4000], out=[flat[:4000]])     # behind it
+  assert (outs[0] == 1.0).all()
+  outs, _ = fused.clip_by_global_norm([flat[:4000]], 1.0, use_norm=keep[7])          # an input that is not written
+  assert (outs[0] == 0.5).all()
+  p, g, v, l2 = (torch.ones(64, device=dev) for _ in range(4))
+  for skip in (p[:2], p[62:], v[3:5]):
+    with pytest.raises(ValueError, match="skip"):
+      fused.clipped_sgd_momentum_l2(p, g, v, l2, 0.1, 0.9, 1.0, skip=skip)
+  assert (p == 1).all() and (v == 1).all()
