@@ -174,12 +174,22 @@ __device__ __forceinline__ void store_row(void* to, int64_t at, int c, int C, co
   store8<DT, NT, ODD>(p, c, C, f);
 }
 
-// fp32 rows take the library's exponential and a true division, 16-bit rows the hardware's (their error, a few
-// 2^-22, vanishes in the rounding of the result).
-template <int DT>
-__device__ __forceinline__ float sigmoid_f(float g) {
-  if constexpr (DT == DT_F32) return 1.f / (1.f + expf(-g));
-  else return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+// A sigmoid gate's factor and its derivative, the latter as e / (1 + e)^2 with e = exp(-|g|): a (1 - a) of a rounded a
+// has lost its digits from g = 8 on (6 % at 16, everything at 18).
+//
+// EXACT: the library's exponential and a true division.  The hardware's are off by up to (|g| + 8) 2^-24 of their value.
+// They serve where a 16-bit value per element is gated and the result is rounded to 16 bits again: the forward pass, and
+// in the gradient of a gate per element dy and dgate; the terms of that call's sums over rows carry the same error
+// into dpost_gamma and dpost_beta, next to the 2^-11 or 2^-8 that their 16-bit factors have been rounded by.  A gate of groups
+// is fp32 whatever the rows are: its gradient is computed EXACT.
+struct Sigmoid {
+  float a, slope;
+};
+template <bool EXACT>
+__device__ __forceinline__ Sigmoid sigmoid_f(float g) {
+  const float e = EXACT ? expf(-fabsf(g)) : __expf(-fabsf(g));
+  const float d = EXACT ? 1.f / (1.f + e) : __builtin_amdgcn_rcpf(1.f + e);
+  return Sigmoid{g < 0.f ? e * d : d, e * d * d};
 }
 
 // v + v of the lane that is `O` away, in every lane (O = 1, 2, 4 .. 32 in this order: from O = 4 on the lanes of the
@@ -381,7 +391,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, fwd_waves(DT, LAYER, K)) void fwd
           else unpack8<DT>(in.gate[k], g[k]);
           if (p.sigmoid) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
+            for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT == DT_F32>(g[k][j]).a;
           }
         }
       }
@@ -719,7 +729,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
         load8<DT_F32>(row_g, c[k], C, g[k]);
         if (p.sigmoid) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<DT>(g[k][j]);
+          for (int j = 0; j < 8; ++j) g[k][j] = sigmoid_f<true>(g[k][j]).a;
         }
       }
     }
@@ -832,8 +842,9 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
             acc[GATE][k][j] += dg[j];
           } else if (element) {
             if (p.sigmoid) {
-              a[j] = sigmoid_f<DT>(a[j]);
-              dg[j] *= a[j] * (1.f - a[j]);
+              const Sigmoid sg = sigmoid_f<DT == DT_F32>(a[j]);
+              a[j] = sg.a;
+              dg[j] *= sg.slope;
             }
             dn *= a[j];
           }
@@ -911,8 +922,9 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
 #pragma unroll
           for (int k = 0; k < K; ++k) {
             if (p.sigmoid) {
+              load8<DT_F32>(reinterpret_cast<const float*>(p.gate) + (int64_t)group * p.ldgate, c[k], C, g[k]);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) acc[GATE][k][j] *= g[k][j] * (1.f - g[k][j]);
+              for (int j = 0; j < 8; ++j) acc[GATE][k][j] *= sigmoid_f<true>(g[k][j]).slope;
             }
             store8<DT_F32>(reinterpret_cast<float*>(p.dgate) + (int64_t)group * C, c[k], C, acc[GATE][k]);
           }
@@ -920,10 +932,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd
       } else if constexpr (!WIDE) {
         over_slots<LPR>(acc[GATE][0], join, [&](int col, float sum) {
           if (col >= C) return;
-          if (p.sigmoid) {
-            const float sg = sigmoid_f<DT>(reinterpret_cast<const float*>(p.gate)[(int64_t)group * p.ldgate + col]);
-            sum *= sg * (1.f - sg);
-          }
+          if (p.sigmoid)
+            sum *= sigmoid_f<true>(reinterpret_cast<const float*>(p.gate)[(int64_t)group * p.ldgate + col]).slope;
           reinterpret_cast<float*>(p.dgate)[(int64_t)group * C + col] = sum;
         });
       }
@@ -963,6 +973,7 @@ struct Finish {
 };
 constexpr int FEW_PARTS = 32;
 
+// (a template so that every element type's file has its own)
 template <int DT>
 __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
   __shared__ float join[32][33];
@@ -986,10 +997,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
       float sum = 0.f;
 #pragma unroll 4
       for (int r = 0; r < f.parts; ++r) sum += from[(int64_t)r * f.C];
-      if (f.sigmoid) {
-        const float sg = sigmoid_f<DT>(f.gate[(int64_t)group * f.ldgate + col]);
-        sum *= sg * (1.f - sg);
-      }
+      if (f.sigmoid) sum *= sigmoid_f<true>(f.gate[(int64_t)group * f.ldgate + col]).slope;
       f.to[4][(int64_t)group * f.C + col] = sum;
       return;
     }
@@ -1010,10 +1018,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
     sum = 0.f;
 #pragma unroll
     for (int q = 0; q < 32; ++q) sum += join[q][threadIdx.x];
-    if (i == 4 && f.sigmoid) {
-      const float sg = sigmoid_f<DT>(f.gate[(int64_t)group * f.ldgate + col]);
-      sum *= sg * (1.f - sg);
-    }
+    if (i == 4 && f.sigmoid) sum *= sigmoid_f<true>(f.gate[(int64_t)group * f.ldgate + col]).slope;
     f.to[i][(int64_t)group * f.C + col] = sum;
   }
 }

@@ -146,8 +146,10 @@ def _gate_factor(gate, rows, channels, group_rows, sigmoid):
   g = g.repeat_interleave(group_rows, 0) if group_rows else g[:rows]
   if not sigmoid:
     return g, 1.0
-  a = torch.sigmoid(g)
-  return a, a * (1 - a)
+  # (a * (1 - a) of a rounded a loses its digits where the gate is open)
+  e = torch.exp(-g.abs())
+  d = 1 / (1 + e)
+  return torch.where(g < 0, e * d, d), e * d * d
 
 
 def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, post_gamma=None, post_beta=None, gate=None,

@@ -539,3 +539,39 @@ def test_gpu_as_entries_of_a_launch_plan():
     native.run_op("residual_norm_bwd", dict(common, h=h.data_ptr(), dh=t["dh"].data_ptr(), dz=t["dz"].data_ptr(),
                                             dx=dx.data_ptr(), dy=dy.data_ptr(), dgate=dg.data_ptr(),
                                             dpost_gamma=v[0].data_ptr(), dpre_gamma=v[1].data_ptr()))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,channels,groups", [
+    (50, 16, 0), (21, 1001, 0), (40, 16, 20), (1500, 16, 500), (6000, 16, 2), (2048, 64, 4), (300, 600, 3), (30, 520, 30),
+    (9000, 48, 1), (12, 5001, 4)])
+def test_gradient_of_open_and_closed_sigmoid_gates(dev, dtype, rows, channels, groups):
+  """Gates far from zero, whose slope is as small as e^-|g|: gradients relative to their own size.
+
+  Without norms up = dh, n = y and dgate = sum over the group's rows of 0.5 dh y times the slope; all terms positive.  The
+  slope sees the exponential ((|g| + 8) U with the hardware's), a sum, a reciprocal and two products: (|g| + 16) U; dgate
+  the terms' product, the last one and the sum's serial roundings besides.  A place adds at most 512 rows in turn, the joins
+  behind it under 64, blocks of long groups rows / 256.  dy = 0.5 dh a: (|g| + 16) U.  Half a step for the result's type; what
+  falls below the smallest normal of that type is off by one of its smallest steps."""
+  gen = torch.Generator().manual_seed(rows + channels)
+  dh = (1000 + 2000 * torch.rand(rows, channels, generator=gen)).to(dtype).to(dev)
+  y = (10 + 20 * torch.rand(rows, channels, generator=gen)).to(dtype).to(dev)
+  values = torch.tensor([8.0, -8.0, 12.0, -12.0, 16.0, -16.0, 18.0, -18.0, 0.0, 20.0, -30.0, 2.5])
+  n = groups or rows
+  gate = values[(torch.arange(n * channels) * 5) % 12].view(n, channels).to(torch.float32 if groups else dtype).to(dev)
+  out = fused.residual_norm_grad(dh, None, y, y, gate=gate, gate_act="sigmoid", residual_scale=0.5)
+  g = gate.double().cpu()
+  slope = 1 / (2 + torch.exp(g) + torch.exp(-g))
+  per = 0.5 * dh.double().cpu() * y.double().cpu()
+  want = (per.view(groups, -1, channels).sum(1) if groups else per) * slope
+  depth = 576 + rows / 256 if groups else 0
+  limit = half_step(gate.dtype) * (1 + 1e-6) + (depth + 32 + g.abs()) * U
+  f = torch.finfo(gate.dtype)
+  assert out["dgate"].dtype == gate.dtype
+  assert ((out["dgate"].double().cpu() - want).abs() <= limit * want + f.smallest_normal * f.eps).all()
+  a = torch.sigmoid(g).repeat_interleave(rows // n, 0)
+  want = 0.5 * dh.double().cpu() * a
+  limit = half_step(dtype) * (1 + 1e-6) + (16 + g.abs().repeat_interleave(rows // n, 0)) * U
+  f = torch.finfo(dtype)
+  assert ((out["dy"].double().cpu() - want).abs() <= limit * want + f.smallest_normal * f.eps).all()
