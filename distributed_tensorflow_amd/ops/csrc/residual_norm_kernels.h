@@ -475,8 +475,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, fwd_waves(DT, LAYER, K)) void fwd
 // A lane keeps its channels for all of its block's rows, so the sums over rows are registers; blocks leave one row of
 // partial sums each and finish_kernel adds them in a fixed order (no atomics: the same bits every time).
 //
-// A block's rows lie in one group (of rows that share a gate row), or it owns whole groups; where a group has fewer
-// rows than the block has row slots, every slot owns whole groups of its own (`own_groups`).
+// A block's rows lie in one group (of rows that share a gate row), or it owns whole groups; many groups of few rows each go
+// to the row slots, each of which owns whole groups (`own_groups`).
 
 struct BwdPlan {
   int blocks;        // grid
@@ -537,9 +537,15 @@ inline BwdPlan plan_bwd(const ResidualNormParams& p, bool full) {
   // others want all that are resident where their groups are many (12544 x 2047: 81 us, 90 with eight).
   const int resident = 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2);
   const int want = 256 * std::max(1, (b.nt && full ? 4 : b.nt && grouped ? resident : 8) / waves);
-  b.own_groups = grouped && slots > 1 && b.group_rows < 4 * slots;
+  // A slot that walks a group by itself takes 0.7 us a row however idle the rest is; a block that shares a group's rows
+  // among its slots pays for joining them, about four rows' time a group.  bf16, 16 channels: 500 rows in one group 364 us a slot
+  // for itself and 8.6 us shared, 4 x 256 10.4 and 10.9, 16 x 2000 20 and 26, 32 x 2000 33 and 26, 16 x 16000 25 and 78.
+  // Long groups of their own also read far apart: 100 x 16000 303 and 166.
+  const int sets = (b.groups + slots - 1) / slots;
+  const int64_t alone = (int64_t)b.group_rows * ((sets + want - 1) / want);
+  b.own_groups = grouped && slots > 1 && b.group_rows < 4 * slots && b.group_rows <= 32 &&
+                 alone <= 4 * (int64_t)((b.groups + want - 1) / want);
   if (b.own_groups) {
-    const int sets = (b.groups + slots - 1) / slots;
     b.blocks = sets < want ? sets : want;
     b.parts = 1;
     return b;

@@ -575,3 +575,34 @@ def test_gradient_of_open_and_closed_sigmoid_gates(dev, dtype, rows, channels, g
   limit = half_step(dtype) * (1 + 1e-6) + (16 + g.abs().repeat_interleave(rows // n, 0)) * U
   f = torch.finfo(dtype)
   assert ((out["dy"].double().cpu() - want).abs() <= limit * want + f.smallest_normal * f.eps).all()
+
+
+def test_few_groups_are_spread_over_the_grid():
+  """Groups that do not fill the row slots of a block share the slots, and their parts several blocks; only many short
+  ones go to a slot each.  (A block leaves five rows of partial sums.)"""
+  from distributed_tensorflow_amd.ops import native
+  if not native.available():
+    pytest.skip("no native extension")
+  blocks = lambda rows, c, group_rows: native.ext().residual_norm_workspace_floats(rows, c, group_rows, 0, 0) // (5 * c)
+  for c in (16, 64, 200):                         # 128, 32 and 8 slots
+    slots = {16: 128, 64: 32, 200: 8}[c]
+    for groups in (1, 2, 7):
+      for per in (4 * slots - 1, slots + 1, 40):
+        assert blocks(groups * per, c, per) >= groups * min(-(-per // slots), 4), (c, groups, per)
+    for groups, per in ((20_000, 1), (20_000, 2), (20_000, 16)):
+      sets = -(-groups // slots)                  # 512 blocks fill the grid, 768 that of a sweep past the caches
+      assert blocks(groups * per, c, per) in (min(sets, 512), min(sets, 768)), (c, groups, per)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,groups,channels", [
+    (511, 1, 16), (510, 2, 16), (2555, 5, 16), (127, 1, 64), (254, 2, 64), (31, 1, 200), (93, 3, 200), (66, 2, 512),
+    (20_000, 5000, 16), (16_000, 1000, 24), (32_000, 1000, 16), (33_000, 1000, 16), (4800, 300, 200)])
+@pytest.mark.parametrize("norm,act", [("rms", "sigmoid"), ("layer", "none")])
+def test_gate_of_few_long_and_many_short_groups(dev, dtype, rows, groups, channels, norm, act):
+  """On either side of the rule that gives groups to slots."""
+  t, kw = make(dev, rows, channels, dtype, norm, gate="group", groups=groups)
+  kw["gate_act"] = act
+  check_forward(t, kw, *fused.residual_norm(t["x"], t["y"], **kw))
+  check_grad(t, kw, fused.residual_norm_grad(t["dh"], t["dz"], t["x"], t["y"], **kw))
