@@ -47,23 +47,41 @@ def _includes():
           "-I" + os.path.join(torch, "include")]
 
 
-def _stale(target, deps):
+def _stale(target, deps, cmd):
+  """Whether `target` is missing, older than what it is made of, or was made by another command: objects of other
+  flags are not linked with today's."""
   if not os.path.exists(target):
     return True
   t = os.path.getmtime(target)
-  return any(os.path.getmtime(d) > t for d in deps)
+  if any(os.path.getmtime(d) > t for d in deps):
+    return True
+  try:
+    with open(_command_file(target)) as f:
+      return f.read() != "\n".join(cmd)
+  except OSError:
+    return True
+
+
+def _command_file(target):
+  return os.path.join(OBJ, os.path.basename(target) + ".cmd")
+
+
+def _run(cmd, target, what):
+  r = subprocess.run(cmd, capture_output=True, text=True)
+  if r.returncode != 0:
+    raise RuntimeError("%s:\n%s\n%s" % (what, r.stdout, r.stderr))
+  with open(_command_file(target), "w") as f:
+    f.write("\n".join(cmd))
 
 
 def _compile(src, force):
   obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
   deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS + OWN_HEADERS.get(src, [])]
-  if not force and not _stale(obj, deps):
-    return obj, False
   cmd = ["hipcc", "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden"] + NO_PACKED_FP32 + [
       "-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj] + _includes()
-  r = subprocess.run(cmd, capture_output=True, text=True)
-  if r.returncode != 0:
-    raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
+  if not force and not _stale(obj, deps, cmd):
+    return obj, False
+  _run(cmd, obj, "hipcc failed for " + src)
   return obj, True
 
 
@@ -75,12 +93,11 @@ def build_data(force: bool = False, verbose: bool = True) -> str:
   """Host-only module `_dtf_data` (input pipeline): plain g++, no GPU code."""
   src = os.path.join(CSRC, "data_loader.cpp")
   target = data_so_path()
-  if force or _stale(target, [src, os.path.join(CSRC, "jpeg_region.h")]):
-    cmd = ["g++", "-O3", "-std=c++17", "-shared", "-fPIC", "-pthread", "-fvisibility=hidden",
-           src, "-o", target, "-ldl"] + _includes()
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-      raise RuntimeError("g++ failed for data_loader.cpp:\n%s\n%s" % (r.stdout, r.stderr))
+  cmd = ["g++", "-O3", "-std=c++17", "-shared", "-fPIC", "-pthread", "-fvisibility=hidden",
+         src, "-o", target, "-ldl"] + _includes()
+  os.makedirs(OBJ, exist_ok=True)
+  if force or _stale(target, [src, os.path.join(CSRC, "jpeg_region.h")], cmd):
+    _run(cmd, target, "g++ failed for data_loader.cpp")
     if verbose:
       print("built", target)
   elif verbose:
@@ -95,11 +112,9 @@ def build(force: bool = False, jobs: int = 4, verbose: bool = True) -> str:
     results = list(ex.map(lambda s: _compile(s, force), SOURCES))
   objs = [o for o, _ in results]
   target = so_path()
-  if force or any(c for _, c in results) or _stale(target, objs):
-    cmd = ["hipcc", "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", target] + objs
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-      raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+  cmd = ["hipcc", "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", target] + objs
+  if force or any(c for _, c in results) or _stale(target, objs, cmd):
+    _run(cmd, target, "link failed")
     if verbose:
       print("built", target)
   elif verbose:
