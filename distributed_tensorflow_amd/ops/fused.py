@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import Dict, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 __all__ = ["sgd_momentum_l2", "clipped_sgd_momentum_l2", "TensorTable", "global_norm", "clip_by_global_norm",
            "residual_norm", "residual_norm_grad"]
@@ -126,6 +127,16 @@ def _no_graph(*tensors):
       if t is not None and t.requires_grad:
         raise ValueError("an argument requires a gradient: it is computed by residual_norm_grad, call under "
                          "torch.no_grad()")
+  _no_tangent(*tensors)
+
+
+def _no_tangent(*tensors):
+  """A forward-mode derivative that an argument carries is refused, not lost (whether or not gradients are recorded)."""
+  if forward_ad._current_level < 0:      # outside of forward_ad.dual_level() and torch.func.jvp
+    return
+  for t in tensors:
+    if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+      raise ValueError("an argument carries a forward-mode derivative, which is not computed here")
 
 
 def _normalised(v: torch.Tensor, layer: bool, eps: float):
@@ -394,6 +405,7 @@ def global_norm(tensors) -> torch.Tensor:
   Squares are summed in 64 bits in a fixed order; nothing is read back to the host, and no graph is recorded.
   """
   t = _table(tensors)
+  _no_tangent(*t.tensors)
   if t.device.type != "cuda":
     return _squares(t.tensors).sqrt().float()
   from . import native  # pylint: disable=import-outside-toplevel
@@ -420,6 +432,7 @@ def clip_by_global_norm(tensors, clip_norm: float, use_norm: Optional[torch.Tens
     tensors = list(tensors)
     t = TensorTable(tensors, [torch.empty_like(x, memory_format=torch.contiguous_format) for x in tensors]
                     if out is None else out, _kept=False)
+  _no_tangent(*t.tensors, *t.out, use_norm)
   if t._clash:
     raise ValueError("outputs overlap each other, or another tensor's input")
   if use_norm is not None and (use_norm.dtype != torch.float32 or use_norm.numel() != 1
@@ -452,6 +465,7 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
   The norm is that of the whole gradient, the regulariser's part included.  `skip` as in `sgd_momentum_l2`: with a
   flag that is set nothing is updated.  A norm that is not finite, without `skip`, makes parameters and velocity NaN.
   """
+  _no_tangent(params, grads, velocity, l2x2)
   n = params.numel()
   for name, t in (("params", params), ("grads", grads), ("velocity", velocity), ("l2x2", l2x2)):
     if t.dtype != torch.float32 or not t.is_contiguous() or t.device != params.device:

@@ -812,3 +812,22 @@ def test_scalars_that_lie_in_an_output_are_refused(dev):
     with pytest.raises(ValueError, match="skip"):
       fused.clipped_sgd_momentum_l2(p, g, v, l2, 0.1, 0.9, 1.0, skip=skip)
   assert (p == 1).all() and (v == 1).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_forward_mode_derivatives_are_refused(dev):
+  from torch.autograd import forward_ad
+  a, b, v, l2 = (torch.randn(16, device=dev) for _ in range(4))
+  with forward_ad.dual_level():
+    fused.clip_by_global_norm([a, b], 1.0)
+    d = forward_ad.make_dual(a.clone(), b)
+    with pytest.raises(ValueError, match="forward-mode"):
+      fused.global_norm([b, d])
+    with pytest.raises(ValueError, match="forward-mode"):
+      fused.clip_by_global_norm([b, d], 1.0)
+    with pytest.raises(ValueError, match="forward-mode"):
+      fused.clip_by_global_norm([b], 1.0, out=[d])
+    with pytest.raises(ValueError, match="forward-mode"):
+      fused.clip_by_global_norm([a], 1.0, use_norm=forward_ad.make_dual(torch.ones((), device=dev), torch.ones((), device=dev)))
+    with pytest.raises(ValueError, match="forward-mode"):
+      fused.clipped_sgd_momentum_l2(d, b, v, l2, 0.1, 0.9, 1.0)

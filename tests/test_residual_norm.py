@@ -606,3 +606,26 @@ def test_gate_of_few_long_and_many_short_groups(dev, dtype, rows, groups, channe
   kw["gate_act"] = act
   check_forward(t, kw, *fused.residual_norm(t["x"], t["y"], **kw))
   check_grad(t, kw, fused.residual_norm_grad(t["dh"], t["dz"], t["x"], t["y"], **kw))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(dev, grad):
+  from torch.autograd import forward_ad
+  t, kw = make(dev, 6, 16, torch.float32, "layer", gate="element")
+  with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+    fused.residual_norm(t["x"], t["y"], **kw)                    # a level alone is nothing
+    dual = lambda v: forward_ad.make_dual(v, torch.ones_like(v))
+    for n in ("x", "y"):
+      with pytest.raises(ValueError, match="forward-mode"):
+        fused.residual_norm(**dict({a: t[a] for a in ("x", "y")}, **{n: dual(t[n])}), **kw)
+    for n in VECTORS + ("gate",):
+      with pytest.raises(ValueError, match="forward-mode"):
+        fused.residual_norm(t["x"], t["y"], **dict(kw, **{n: dual(kw[n])}))
+    for i in range(4):
+      args = [t["dh"], t["dz"], t["x"], t["y"]]
+      args[i] = dual(args[i])
+      with pytest.raises(ValueError, match="forward-mode"):
+        fused.residual_norm_grad(*args, **kw)
+  with pytest.raises(ValueError, match="forward-mode"):
+    torch.func.jvp(lambda v: fused.residual_norm(v, t["y"], **kw), (t["x"],), (t["x"],))
