@@ -81,6 +81,11 @@ def _elsewhere(index: int) -> bool:
   return index != torch.cuda.current_device()
 
 
+# Kernels write through addresses, which autograd does not see: without this a backward pass would use a tensor that it
+# has saved and that was overwritten since, instead of refusing it.
+_written = torch.autograd.graph.increment_version
+
+
 # raw hipStream_t of a device's current stream, without a Stream object (0.1 instead of 2.8 us)
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -99,6 +104,7 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
   ext().clipped_sgd(params.data_ptr(), grads.data_ptr(), velocity.data_ptr(), l2x2.data_ptr(), n, lr, momentum,
                     grad_scale, clip_norm, skip.data_ptr() if skip is not None else 0, ws.data_ptr(),
                     norm.data_ptr(), _current_stream(index))
+  _written([params, velocity] if momentum else [params])
   return norm
 
 
@@ -160,8 +166,10 @@ def clip_list_scale(table, clip_norm: float, use_norm: Optional[torch.Tensor]) -
   resident, norm, ws = _clip_list_launch(table, stream)
   if use_norm is not None:
     table.list.clip(resident, 0, use_norm.data_ptr(), clip_norm, 0, stream)
-    return use_norm
-  table.list.clip(resident, ws.data_ptr(), 0, clip_norm, norm.data_ptr(), stream)
+    norm = use_norm
+  else:
+    table.list.clip(resident, ws.data_ptr(), 0, clip_norm, norm.data_ptr(), stream)
+  _written(table.out)
   return norm
 
 

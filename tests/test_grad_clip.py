@@ -831,3 +831,33 @@ def test_forward_mode_derivatives_are_refused(dev):
       fused.clip_by_global_norm([a], 1.0, use_norm=forward_ad.make_dual(torch.ones((), device=dev), torch.ones((), device=dev)))
     with pytest.raises(ValueError, match="forward-mode"):
       fused.clipped_sgd_momentum_l2(d, b, v, l2, 0.1, 0.9, 1.0)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("table", [True, False])
+def test_autograd_sees_what_was_overwritten(dev, table):
+  """A backward pass that has saved a tensor which was clipped or updated in place since is refused, as after any
+  in-place operation; what was only read is as it was."""
+  a, w = torch.randn(50, device=dev), torch.randn(50, device=dev, requires_grad=True)
+  def product():
+    return (a * w).sum()
+
+  for use_norm in (None, torch.tensor(2.0, device=dev)):
+    loss = product()
+    fused.global_norm([a])
+    fused.clip_by_global_norm([a], 1.0)                      # into a new tensor
+    loss.backward()
+    loss = product()
+    t = fused.TensorTable([a]) if table else [a]
+    fused.clip_by_global_norm(t, 0.5, use_norm=use_norm, **({} if table else dict(out=t)))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+      loss.backward()
+  p, g, v, l2 = (torch.randn(50, device=dev) for _ in range(4))
+  before = [t._version for t in (p, g, v, l2)]
+  fused.clipped_sgd_momentum_l2(p, g, v, l2, 0.1, 0.9, 1.0)
+  assert [t._version > b for t, b in zip((p, g, v, l2), before)] == [True, False, True, False]
+  before = v._version
+  fused.clipped_sgd_momentum_l2(p, g, v, l2, 0.1, 0.0, 1.0)
+  assert v._version == before
+  with torch.inference_mode():                                # such tensors have no versions
+    fused.clip_by_global_norm([torch.ones(5, device=dev)], 0.1)
