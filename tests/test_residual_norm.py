@@ -629,3 +629,29 @@ def test_forward_mode_derivatives_are_refused(dev, grad):
         fused.residual_norm_grad(*args, **kw)
   with pytest.raises(ValueError, match="forward-mode"):
     torch.func.jvp(lambda v: fused.residual_norm(v, t["y"], **kw), (t["x"],), (t["x"],))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("channels", [64, 4096, 5000, 8192])
+def test_the_largest_values_a_row_may_hold(dev, dtype, norm, channels):
+  """Squares sum to float32's largest number, sqrt(2^128 / channels) a value: a tenth below, rows are right; above (an
+  eighth, past the 2^-9 that bf16 may round down and what centring takes off) their normalised values are zero, as stated."""
+  gen = torch.Generator().manual_seed(channels)
+  limit = (2.0 ** 128 / channels) ** 0.5
+  sign = (torch.rand(2, channels, generator=gen) < 0.5).float() * 2 - 1
+  sign[:, channels // 2:] = -sign[:, :channels // 2]              # as many of either: a mean of zero
+  gamma, dz = 1 + 0.3 * torch.randn(channels, generator=gen), torch.randn(2, channels, generator=gen).to(dtype)
+  x = (sign * (limit * torch.tensor([[0.9], [1.125]]))).to(dtype)
+  gamma, dz, x = gamma.to(dev), dz.to(dev), x.to(dev)
+  h, z = fused.residual_norm(x, pre_gamma=gamma, norm=norm)
+  assert h is x
+  want = norm64(x[:1].double().cpu(), gamma.double().cpu(), None, norm, 1e-6)[0]
+  limit_z = half_step(dtype) * want.abs() + 128 * U * (want.abs().max() + 1)
+  assert ((z[:1].double().cpu() - want).abs() <= limit_z).all()
+  assert (z[1] == 0).all()
+  out = fused.residual_norm_grad(None, dz, x, pre_gamma=gamma, norm=norm)
+  want = dz[0].double().cpu() * want[0] / gamma.double().cpu()       # the second row's share is nothing
+  assert ((out["dpre_gamma"].double().cpu() - want).abs() <= 256 * U * (want.abs().max() + 1)).all()
+  assert torch.isfinite(out["dx"].float()).all()
