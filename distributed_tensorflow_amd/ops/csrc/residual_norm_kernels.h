@@ -488,8 +488,11 @@ struct BwdPlan {
 };
 
 // Waves per SIMD that the backward kernel is built for: its registers (sums over rows, vectors, a row in work and the
-// next ones' loads) leave room for two, three for RMS norms of 16-bit rows.
-constexpr int bwd_waves(int dt, bool layer, int chunks) { return !layer && dt != DT_F32 && chunks == 1 ? 3 : 2; }
+// next ones' loads) leave room for two, three for RMS norms of 16-bit rows.  (A FULL kernel with the sums of a group's
+// gate besides would spill 6 - 12 registers at three, and its grids ask for two at most.)
+constexpr int bwd_waves(int dt, bool layer, int chunks, int mode) {
+  return !layer && dt != DT_F32 && chunks == 1 && mode != FULL_GROUP ? 3 : 2;
+}
 
 inline int narrow_lanes(int C) {       // lanes a row of up to 512 channels
   int l = 2;
@@ -535,7 +538,7 @@ inline BwdPlan plan_bwd(const ResidualNormParams& p, bool full) {
   // two rows under way, run large sweeps best as a front of four (200704 x 512 with a gate per element: 277 us, 306 with
   // eight; the last ResNet stage with a gate per image: 66 and 69, and a group's gate gradient stays in one block); the
   // others want all that are resident where their groups are many (12544 x 2047: 81 us, 90 with eight).
-  const int resident = 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2);
+  const int resident = 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2, ANY_GROUP);
   const int want = 256 * std::max(1, (b.nt && full ? 4 : b.nt && grouped ? resident : 8) / waves);
   // A slot that walks a group by itself takes 0.7 us a row however idle the rest is; a block that shares a group's rows
   // among its slots pays for joining them, about four rows' time a group.  bf16, 16 channels: 500 rows in one group 364 us a slot
@@ -662,7 +665,7 @@ __device__ __forceinline__ void over_slots(const float* v, float* join, F use) {
 }
 
 template <int DT, int LPR, bool WIDE, int K, bool LAYER, int MODE, bool NT>
-__global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K)) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
+__global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K, MODE)) void bwd_kernel(const ResidualNormParams p, const BwdPlan plan,
                                                                const Partials part) {
   typedef typename Elem<DT>::T T;
   constexpr bool FULL = MODE >= FULL_PLAIN, GROUP = MODE == ANY_GROUP || MODE == FULL_GROUP, ODD = !FULL;
