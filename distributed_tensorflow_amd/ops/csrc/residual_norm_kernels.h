@@ -473,7 +473,9 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, fwd_waves(DT, LAYER, K)) void fwd
 // (the bracketed means only with `layer`).  The statistics are taken again from h and y, which are in registers
 // anyway: two sums more per row instead of saved tensors that could belong to another call.
 // A lane keeps its channels for all of its block's rows, so the sums over rows are registers; blocks leave one row of
-// partial sums each and finish_kernel adds them in a fixed order (no atomics: the same bits every time).
+// partial sums each and finish_kernel adds them in a fixed order (no atomics: the same bits every time).  A slot's sum over
+// its rows is fp32 and so is a block's partial sum in memory; both joins add in 64 bits (131072 x 16 fp32 layer: 8.1e-8 off, as
+// 64-bit sums over fp32 terms are, 1.9e-7 with fp32 joins; 1 % of the time of small calls).
 //
 // A block's rows lie in one group (of rows that share a gate row), or it owns whole groups; many groups of few rows each go
 // to the row slots, each of which owns whole groups (`own_groups`).
@@ -631,7 +633,8 @@ __device__ __forceinline__ void load_full(RowIn<DT, K>& in, const ResidualNormPa
 }
 
 // Sums the slots' eight channels a lane and hands every column's sum to `use(column, sum)`.  A thread adds eight slots,
-// then the eighths are added (one thread a column and all 128 slots in turn took 1 us a vector for 16 channels).
+// then the eighths are added (one thread a column and all 128 slots in turn took 1 us a vector for 16 channels).  In
+// 64 bits: `sum` is rounded where it is stored, and `join` holds the eighths as doubles.
 template <int LPR, typename F>
 __device__ __forceinline__ void over_slots(const float* v, float* join, F use) {
   constexpr int COLS = LPR * 8, PARTS = COLS >= 256 ? 1 : 256 / COLS, SLOTS = 256 / LPR;
@@ -642,23 +645,24 @@ __device__ __forceinline__ void over_slots(const float* v, float* join, F use) {
   if constexpr (PARTS == 1) {
 #pragma unroll
     for (int col = threadIdx.x; col < COLS; col += 256) {
-      float sum = 0.f;
+      double sum = 0.;
 #pragma unroll
       for (int q = 0; q < SLOTS; ++q) sum += join[q * COLS + col];
       use(col, sum);
     }
   } else {
     const int col = threadIdx.x % COLS, part = threadIdx.x / COLS;
-    float sum = 0.f;
+    double sum = 0.;
 #pragma unroll
     for (int q = 0; q < SLOTS / PARTS; ++q) sum += join[(part * (SLOTS / PARTS) + q) * COLS + col];
     __syncthreads();
-    join[threadIdx.x] = sum;
+    double* parts = reinterpret_cast<double*>(join);
+    parts[threadIdx.x] = sum;
     __syncthreads();
     if (part == 0) {
-      sum = 0.f;
+      sum = 0.;
 #pragma unroll
-      for (int q = 0; q < PARTS; ++q) sum += join[q * COLS + col];
+      for (int q = 0; q < PARTS; ++q) sum += parts[q * COLS + col];
       use(col, sum);
     }
   }
@@ -675,7 +679,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K, MODE)) vo
   constexpr int SUMS = 2 + (LAYER ? 2 : 0) + (GROUP ? 1 : 0), GATE = SUMS - 1;
   __shared__ Red red;
   clear_red<WIDE>(red);
-  __shared__ float join[WIDE ? 1 : 256 * 8];
+  __shared__ __attribute__((aligned(8))) float join[WIDE ? 2 : 256 * 8];
   int turn = 0;
   const int lanes = WIDE ? (int)blockDim.x : LPR;
   const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x % LPR);
@@ -939,11 +943,11 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K, MODE)) vo
           }
         }
       } else if constexpr (!WIDE) {
-        over_slots<LPR>(acc[GATE][0], join, [&](int col, float sum) {
+        over_slots<LPR>(acc[GATE][0], join, [&](int col, double sum) {
           if (col >= C) return;
           if (p.sigmoid)
             sum *= sigmoid_f<true>(reinterpret_cast<const float*>(p.gate)[(int64_t)group * p.ldgate + col]).slope;
-          reinterpret_cast<float*>(p.dgate)[(int64_t)group * C + col] = sum;
+          reinterpret_cast<float*>(p.dgate)[(int64_t)group * C + col] = (float)sum;
         });
       }
 #pragma unroll
@@ -962,8 +966,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, bwd_waves(DT, LAYER, K, MODE)) vo
 #pragma unroll
       for (int k = 0; k < K; ++k) store8<DT_F32>(to, c[k], C, acc[i][k]);
     } else {
-      over_slots<LPR>(acc[i][0], join, [&](int col, float sum) {
-        if (col < C) to[col] = sum;
+      over_slots<LPR>(acc[i][0], join, [&](int col, double sum) {
+        if (col < C) to[col] = (float)sum;
       });
     }
   }
@@ -985,7 +989,7 @@ constexpr int FEW_PARTS = 32;
 // (a template so that every element type's file has its own)
 template <int DT>
 __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
-  __shared__ float join[32][33];
+  __shared__ double join[32][33];
   const int cols = (f.C + 31) / 32;
   int b = (int)blockIdx.x, i = 4, group = 0, rows = f.parts, col;
   if (b < f.vector_blocks) {
@@ -1003,11 +1007,11 @@ __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
       col = (b % wide_cols) * 1024 + (int)threadIdx.x;
       if (col >= f.C) return;
       const float* from = f.from[4] + (int64_t)group * f.parts * f.C + col;
-      float sum = 0.f;
+      double sum = 0.;
 #pragma unroll 4
       for (int r = 0; r < f.parts; ++r) sum += from[(int64_t)r * f.C];
       if (f.sigmoid) sum *= sigmoid_f<true>(f.gate[(int64_t)group * f.ldgate + col]).slope;
-      f.to[4][(int64_t)group * f.C + col] = sum;
+      f.to[4][(int64_t)group * f.C + col] = (float)sum;
       return;
     }
     group = b / cols;
@@ -1015,7 +1019,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
   }
   col = b * 32 + (threadIdx.x & 31);
   const int slice = threadIdx.x >> 5;
-  float sum = 0.f;
+  double sum = 0.;
   if (col < f.C) {
     const float* from = f.from[i] + (int64_t)group * f.parts * f.C + col;
 #pragma unroll 16
@@ -1024,11 +1028,11 @@ __global__ __launch_bounds__(1024) void finish_kernel(const Finish f) {
   join[slice][threadIdx.x & 31] = sum;
   __syncthreads();
   if (slice == 0 && col < f.C) {
-    sum = 0.f;
+    sum = 0.;
 #pragma unroll
     for (int q = 0; q < 32; ++q) sum += join[q][threadIdx.x];
     if (i == 4 && f.sigmoid) sum *= sigmoid_f<true>(f.gate[(int64_t)group * f.ldgate + col]).slope;
-    f.to[i][(int64_t)group * f.C + col] = sum;
+    f.to[i][(int64_t)group * f.C + col] = (float)sum;
   }
 }
 

@@ -220,7 +220,8 @@ def residual_norm_grad(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], h
   is).  Returns a dict of dx, dy (the type of h), dgate (the type and shape of gate; a row of a [groups, channels] gate sums
   over its rows), dpost_gamma, dpost_beta, dpre_gamma, dpre_beta (float32 [channels]), None for what was not
   given.  The norms' statistics are taken from h and y again, so nothing has to be kept from the forward call.
-  Sums over rows are float32 in a fixed order: the same call gives the same bits.
+  Sums over rows run in a fixed order, float32 within the few rows that one place on the grid adds up and 64 bits
+  beyond: the same call gives the same bits.
   """
   rows, c, group_rows, ldgate, sigmoid, layer = _seam(h, y, post_gamma, post_beta, gate, gate_act, pre_gamma, pre_beta,
                                                       norm, eps)

@@ -655,3 +655,26 @@ def test_the_largest_values_a_row_may_hold(dev, dtype, norm, channels):
   want = dz[0].double().cpu() * want[0] / gamma.double().cpu()       # the second row's share is nothing
   assert ((out["dpre_gamma"].double().cpu() - want).abs() <= 256 * U * (want.abs().max() + 1)).all()
   assert torch.isfinite(out["dx"].float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,channels", [(131_072, 16), (131_072, 24), (65_536, 64), (20_000, 200), (8192, 512), (16_384, 600)])
+def test_gpu_sums_over_many_rows(rows, channels):
+  """dpre_beta is the sum of dz itself.  With positive terms only the roundings on the way count: those of a slot's own rows,
+  one for a block's partial sum and one for the result; the joins are in 64 bits.  Equal terms of these values would be
+  rounded the same way again and again by joins in 32 (131072 of 16 channels: 8.7 U instead of 3)."""
+  from distributed_tensorflow_amd.ops import native
+  gen = torch.Generator().manual_seed(channels)
+  dz = 1 + torch.rand(rows, channels, generator=gen)
+  dz[:, ::2] = 1 + (5033592 + 144 * torch.arange(0, channels, 2)) / 2.0 ** 23
+  ones = torch.ones(channels, device="cuda")
+  h = torch.randn(rows, channels, generator=gen).cuda()
+  out = fused.residual_norm_grad(None, dz.cuda(), h, pre_gamma=ones, pre_beta=ones, norm="layer")
+  lanes = 2
+  while lanes * 8 < channels:
+    lanes *= 2
+  slots = 256 // lanes if channels <= 512 else 1
+  blocks = native.ext().residual_norm_workspace_floats(rows, channels, 0, 2, 1) // (5 * channels)
+  own = -(-rows // (blocks * slots))
+  want = dz.double().sum(0)
+  assert ((out["dpre_beta"].double().cpu() - want).abs() <= (own - 1 + 2) * U * want * (1 + 1e-6)).all()
