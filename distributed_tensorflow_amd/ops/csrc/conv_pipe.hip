@@ -73,9 +73,9 @@ constexpr int pipe_occ(int bm, int bn, int nw, int bk, int stages, bool inbn = f
   return w > 4 ? 4 : (w < 1 ? 1 : w);
 }
 
-// max(x * scale + shift, 0) of the two 16-bit elements of a dword, rounded back to 16 bits.  bf16: one
-// packed multiply-add for the pair and the ReLU on the packed result (a signed 16-bit max against
-// zero clears every negative value, -0 included) - five vector instructions a pair instead of seven.
+// max(x * scale + shift, 0) of the two 16-bit elements of a dword, rounded back to 16 bits.  bf16: the
+// ReLU on the packed result (a signed 16-bit max against zero clears every negative value, -0
+// included) - six vector instructions a pair instead of seven.
 template <int DT>
 __device__ __forceinline__ uint32_t bn_relu_pair(uint32_t w, float sc_lo, float sc_hi, float sh_lo, float sh_hi) {
   if constexpr (DT == DT_BF16) {

@@ -19,7 +19,7 @@
 // kernel's arguments (a list given as such: nothing to upload and keep alive, and a captured launch holds its own copy), or
 // in device memory (a table that is kept: any number of tensors in one launch).
 //
-// Measured: 161 tensors of 25.6 M fp32 elements 18 + 35 us (5.7 and 5.9 TB/s), 384 of 400 M mixed ones 122 + 295 us (6.6 and
+// Measured: 161 tensors of 25.6 M fp32 elements 18 + 34 us (5.7 and 6.0 TB/s), 384 of 400 M mixed ones 122 + 293 us (6.6 and
 // 5.5 TB/s); what bounds both is memory, and that the norm has to be known before the first element can be scaled.
 #include <algorithm>
 #include <stdexcept>

@@ -15,9 +15,9 @@
 //
 // Loads and stores take any alignment (rows of odd length start anywhere).
 //
-// Measured on the largest sweeps, 200704 x 512 bf16: forward with a gate per image 148 us (5.6 TB/s), gradient with a gate
-// per element 277 us (5.9 TB/s; a copy of 1 GB 5.0); 12544 x 2048 bf16: 36 us (layer, scale per channel) and 62 us (gradient,
-// gate per image); one row of 4096: 3 us.
+// Measured, calls one behind the other: 200704 x 512 bf16 forward with a gate per image 148 us (5.6 TB/s), gradient with a
+// sigmoid gate per element 281 us (5.9 TB/s; a copy of 1 GB 5.0); 12544 x 2048 bf16 forward, layer, scale per channel 40 us,
+// gradient with a gate per image 67 us, of which its two kernels take 61 and 5; one row of 4096 9.8 us, its kernel 3.3.
 //
 // A file per element type instantiates these (residual_norm_bf16 / f16 / f32.hip).
 #pragma once
@@ -538,7 +538,7 @@ inline BwdPlan plan_bwd(const ResidualNormParams& p, bool full) {
   b.nt = big(p, 6);
   // Waves a CU: eight (6000 x 1024 bf16: 25 us, 41 with two; 3000 x 2048 layer: 27.5, 35 with twelve).  FULL kernels, with
   // two rows under way, run large sweeps best as a front of four (200704 x 512 with a gate per element: 277 us, 306 with
-  // eight; the last ResNet stage with a gate per image: 66 and 69, and a group's gate gradient stays in one block); the
+  // eight, before its sigmoid kept its digits; the last ResNet stage with a gate per image: 66 and 69, and a group's gate gradient stays in one block); the
   // others want all that are resident where their groups are many (12544 x 2047: 81 us, 90 with eight).
   const int resident = 4 * bwd_waves(p.dt, p.layer, p.C <= 4096 ? 1 : 2, ANY_GROUP);
   const int want = 256 * std::max(1, (b.nt && full ? 4 : b.nt && grouped ? resident : 8) / waves);
