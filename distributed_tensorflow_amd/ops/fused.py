@@ -7,6 +7,7 @@ library fallback on the device path.
 """
 from __future__ import annotations
 
+import itertools
 from typing import Dict, Optional, Sequence
 
 import torch
@@ -127,14 +128,14 @@ def _no_graph(*tensors):
       if t is not None and t.requires_grad:
         raise ValueError("an argument requires a gradient: it is computed by residual_norm_grad, call under "
                          "torch.no_grad()")
-  _no_tangent(*tensors)
+  _no_tangent(tensors)
 
 
-def _no_tangent(*tensors):
+def _no_tangent(*lists):
   """A forward-mode derivative that an argument carries is refused, not lost (whether or not gradients are recorded)."""
   if forward_ad._current_level < 0:      # outside of forward_ad.dual_level() and torch.func.jvp
     return
-  for t in tensors:
+  for t in itertools.chain(*lists):
     if t is not None and forward_ad.unpack_dual(t).tangent is not None:
       raise ValueError("an argument carries a forward-mode derivative, which is not computed here")
 
@@ -407,7 +408,7 @@ def global_norm(tensors) -> torch.Tensor:
   Squares are summed in 64 bits in a fixed order; nothing is read back to the host, and no graph is recorded.
   """
   t = _table(tensors)
-  _no_tangent(*t.tensors)
+  _no_tangent(t.tensors)
   if t.device.type != "cuda":
     return _squares(t.tensors).sqrt().float()
   from . import native  # pylint: disable=import-outside-toplevel
@@ -421,7 +422,7 @@ def clip_by_global_norm(tensors, clip_norm: float, use_norm: Optional[torch.Tens
   `tensors`: a list, clipped into new tensors or into `out` (a list of the same shapes and types; the list itself:
   in place), or a `TensorTable`, which brings its own.  `use_norm`: a float32 scalar on the device that takes the
   place of the norm (of a model whose gradients are spread over processes).  A norm that is infinite or NaN makes
-  every result NaN; a norm of zero changes nothing.  Nothing is read back to the host.
+  every result NaN; a norm of zero changes nothing.  Nothing is read back to the host, and no graph is recorded.
   """
   clip_norm = float(clip_norm)
   if not clip_norm > 0:
@@ -434,7 +435,7 @@ def clip_by_global_norm(tensors, clip_norm: float, use_norm: Optional[torch.Tens
     tensors = list(tensors)
     t = TensorTable(tensors, [torch.empty_like(x, memory_format=torch.contiguous_format) for x in tensors]
                     if out is None else out, _kept=False)
-  _no_tangent(*t.tensors, *t.out, use_norm)
+  _no_tangent(t.tensors, t.out, (use_norm,))
   if t._clash:
     raise ValueError("outputs overlap each other, or another tensor's input")
   if use_norm is not None and (use_norm.dtype != torch.float32 or use_norm.numel() != 1
@@ -467,7 +468,7 @@ def clipped_sgd_momentum_l2(params: torch.Tensor, grads: torch.Tensor, velocity:
   The norm is that of the whole gradient, the regulariser's part included.  `skip` as in `sgd_momentum_l2`: with a
   flag that is set nothing is updated.  A norm that is not finite, without `skip`, makes parameters and velocity NaN.
   """
-  _no_tangent(params, grads, velocity, l2x2)
+  _no_tangent((params, grads, velocity, l2x2))
   n = params.numel()
   for name, t in (("params", params), ("grads", grads), ("velocity", velocity), ("l2x2", l2x2)):
     if t.dtype != torch.float32 or not t.is_contiguous() or t.device != params.device:
